@@ -6,6 +6,23 @@ use std::os::raw::{c_char, c_void};
 #[repr(C)] pub struct FhipWeight { _private: [u8; 0] }
 #[repr(C)] pub struct FhipPool { _private: [u8; 0] }
 #[repr(C)] pub struct FhipGguf { _private: [u8; 0] }
+/// A paged key/value cache as its entry points take it (read during the call).
+#[repr(C)]
+pub struct FhipPaged {
+    pub ty: u32,
+    pub page_rows: u32,
+    pub n_pages: usize,
+    pub n_kv: usize,
+    pub head_dim: usize,
+    pub d_k: *mut c_void,
+    pub d_v: *mut c_void,
+    pub d_k_scales: *mut c_void,
+    pub d_v_scales: *mut c_void,
+    pub d_table: *const u32,
+    pub n_seq: usize,
+    pub pages_per_seq: usize,
+    pub table_stride: usize,
+}
 
 pub const FHIP_OK: i32 = 0;
 pub const FHIP_ERR_UNSUPPORTED_TYPE: i32 = -1;
@@ -99,6 +116,14 @@ extern "C" {
     pub fn fhip_decode_attention_ex(d_q: *const f32, d_k_cache: *const f32, d_v_cache: *const f32, n_head: usize, n_kv: usize, head_dim: usize, len: usize, d_last_pos: *const u32, window: usize, softcap: f32, d_ws: *mut f32, d_out: *mut f32, stream: *mut c_void) -> i32;
     pub fn fhip_qkv_post_attention(d_qkv: *const f32, d_bias: *const f32, d_q_norm: *const f32, d_k_norm: *const f32, d_pos: *const u32, d_freq_scale: *const f32, n_head: usize, n_kv: usize, head_dim: usize, n_rot: usize, interleaved: i32, eps: f32, base: f32, d_k_cache: *mut f32, d_v_cache: *mut f32, cap: usize, len: usize, window: usize, softcap: f32, d_ws: *mut f32, d_out: *mut f32, stream: *mut c_void) -> i32;
     pub fn fhip_qkv_post_attention_kvq(fmt: i32, d_qkv: *const f32, d_bias: *const f32, d_q_norm: *const f32, d_k_norm: *const f32, d_pos: *const u32, d_freq_scale: *const f32, n_head: usize, n_kv: usize, head_dim: usize, n_rot: usize, interleaved: i32, eps: f32, base: f32, d_k_codes: *mut u32, d_k_scales: *mut u32, d_v_codes: *mut u32, d_v_scales: *mut u32, cap: usize, len: usize, window: usize, softcap: f32, d_ws: *mut f32, d_out: *mut f32, stream: *mut c_void) -> i32;
+    pub fn fhip_paged_append(kv: *const FhipPaged, d_qkv: *const f32, d_bias: *const f32, d_q_norm: *const f32, d_k_norm: *const f32, d_seqs: *const u32, d_positions: *const u32, d_freq_scale: *const f32, t: usize, n_head: usize, n_rot: usize, interleaved: i32, eps: f32, base: f32, d_q_out: *mut f32, stream: *mut c_void) -> i32;
+    pub fn fhip_paged_attention_ws_bytes(kv: *const FhipPaged, n_head: usize, max_len: usize) -> usize;
+    pub fn fhip_paged_attention(kv: *const FhipPaged, d_q: *const f32, d_lens: *const u32, max_len: usize, n_head: usize, window: usize, softcap: f32, d_ws: *mut f32, d_out: *mut f32, stream: *mut c_void) -> i32;
+    pub fn fhip_paged_key_bounds(kv: *const FhipPaged, d_lens: *const u32, d_new: *const u32, max_new: usize, d_bounds: *mut f32, stream: *mut c_void) -> i32;
+    pub fn fhip_paged_select_ws_bytes(kv: *const FhipPaged, max_len: usize) -> usize;
+    pub fn fhip_paged_select(kv: *const FhipPaged, d_q: *const f32, d_lens: *const u32, max_len: usize, d_bounds: *const f32, n_head: usize, n_select: usize, keep_first: usize, keep_last: usize, d_ws: *mut c_void, d_selected: *mut u32, stream: *mut c_void) -> i32;
+    pub fn fhip_paged_attention_selected(kv: *const FhipPaged, d_q: *const f32, d_lens: *const u32, d_selected: *const u32, n_select: usize, n_head: usize, softcap: f32, d_ws: *mut f32, d_out: *mut f32, stream: *mut c_void) -> i32;
+    pub fn fhip_paged_rows(kv: *const FhipPaged, seq: usize, row0: usize, rows: usize, d_k_out: *mut f32, d_v_out: *mut f32, stream: *mut c_void) -> i32;
     pub fn fhip_norm_matmul_q(w: *const FhipWeight, d_x: *const f32, d_resid: *const f32, d_norm_w: *const f32, eps: f32, d_x_out: *mut f32, d_h_scratch: *mut f32, swiglu: i32, d_y: *mut f32, stream: *mut c_void) -> i32;
     pub fn fhip_norm_matmul_q_count(w: *const FhipWeight, d_x: *const f32, d_resid: *const f32, d_norm_w: *const f32, eps: f32, d_x_out: *mut f32, d_h_scratch: *mut f32, swiglu: i32, d_y: *mut f32, d_count: *mut u32, by: u32, stream: *mut c_void) -> i32;
     pub fn fhip_ffn_noalloc(gate_up: *const FhipWeight, down: *const FhipWeight, d_x: *const f32, rows_x: usize, d_y: *mut f32, stream: *mut c_void) -> i32;

@@ -15,6 +15,14 @@ _vp = C.c_void_p
 _sz = C.c_size_t
 _u32 = C.c_uint32
 
+
+
+class Paged(C.Structure):
+    """fhip_paged, a paged key/value cache as its entry points take it."""
+    _fields_ = [("type", _u32), ("page_rows", _u32), ("n_pages", _sz), ("n_kv", _sz), ("head_dim", _sz), ("d_k", _vp), ("d_v", _vp), ("d_k_scales", _vp), ("d_v_scales", _vp),
+                ("d_table", _vp), ("n_seq", _sz), ("pages_per_seq", _sz), ("table_stride", _sz)]
+
+
 # name -> (restype, argtypes); exactly the symbols include/ferric_hip.h declares
 SYMBOLS = {
     "fhip_init": (C.c_int, [C.c_int]),
@@ -124,6 +132,14 @@ SYMBOLS = {
     "fhip_qkv_post_attention": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, C.c_int, C.c_float, C.c_float, _vp, _vp, _sz, _sz, _sz,
                                           C.c_float, _vp, _vp, _vp]),
     "fhip_decode_attention_ex": (C.c_int, [_vp, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _sz, C.c_float, _vp, _vp, _vp]),
+    "fhip_paged_append": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, C.c_int, C.c_float, C.c_float, _vp, _vp]),
+    "fhip_paged_attention_ws_bytes": (_sz, [_vp, _sz, _sz]),
+    "fhip_paged_attention": (C.c_int, [_vp, _vp, _vp, _sz, _sz, _sz, C.c_float, _vp, _vp, _vp]),
+    "fhip_paged_key_bounds": (C.c_int, [_vp, _vp, _vp, _sz, _vp, _vp]),
+    "fhip_paged_select_ws_bytes": (_sz, [_vp, _sz]),
+    "fhip_paged_select": (C.c_int, [_vp, _vp, _vp, _sz, _vp, _sz, _sz, _sz, _sz, _vp, _vp, _vp]),
+    "fhip_paged_attention_selected": (C.c_int, [_vp, _vp, _vp, _vp, _sz, _sz, C.c_float, _vp, _vp, _vp]),
+    "fhip_paged_rows": (C.c_int, [_vp, _sz, _sz, _sz, _vp, _vp, _vp]),
     "fhip_add_count": (C.c_int, [_vp, _vp, _sz, _vp, _vp, _u32, _vp]),
     "fhip_norm_matmul_q_count": (C.c_int, [_vp, _vp, _vp, _vp, C.c_float, _vp, _vp, C.c_int, _vp, _vp, _u32, _vp]),
     "fhip_norm_matmul_q": (C.c_int, [_vp, _vp, _vp, _vp, C.c_float, _vp, _vp, C.c_int, _vp, _vp]),

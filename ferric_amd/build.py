@@ -44,6 +44,7 @@ UNITS = {
     "probe.hip": [],
     "decode_ops.hip": [],
     "prefill_attn.hip": [],
+    "paged.hip": [],
     "gguf.hip": [],
 }
 

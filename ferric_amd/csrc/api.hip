@@ -2,8 +2,10 @@
 // the reference's error behaviour, weight handles, and thin dispatch into the kernel launchers.
 #include "f16x2.hpp"
 #include "hostmem.hpp"
+#include "paged.hpp"
 #include "prompt.hpp"
 
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -1684,6 +1686,141 @@ int fhip_matvec_q8_0_pooled(fhip_pool* p, const float* h_x, size_t x_len, const 
     if ((rc = fhip::launch_gemv(&view, p->d_x, 1, p->d_y, 0, p->stream))) return rc;
     if ((rc = check_hip(hipMemcpyAsync(h_y, p->d_y, rows * sizeof(float), hipMemcpyDeviceToHost, p->stream), "hipMemcpy D2H"))) return rc;
     return check_hip(hipStreamSynchronize(p->stream), "hipStreamSynchronize");
+}
+
+// ---- the paged key/value cache ----------------------------------------------------------------
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// the description's own checks, and how the kernels take it
+static int paged_view(const char* who, const fhip_paged* kv, fhip::PagedView& v) {
+    if (!kv) return set_error(FHIP_ERR_ARG, "%s: NULL cache", who);
+    if (kv->type != FHIP_F32 && kv->type != FHIP_F16 && kv->type != FHIP_BF16 && kv->type != FHIP_Q8_0)
+        return set_error(FHIP_ERR_UNSUPPORTED_TYPE, "%s: a paged cache holds F32, F16, BF16 or Q8_0, not ggml type %u", who, kv->type);
+    if (kv->head_dim != 64 && kv->head_dim != 128) return set_error(FHIP_ERR_SHAPE, "%s: head_dim must be 64 or 128, got %zu", who, kv->head_dim);
+    if (kv->page_rows < 16 || kv->page_rows > 4096 || (kv->page_rows & (kv->page_rows - 1)))
+        return set_error(FHIP_ERR_SHAPE, "%s: page_rows must be a power of two from 16 to 4096, got %u", who, kv->page_rows);
+    if (kv->n_kv < 1 || kv->n_kv > 4096) return set_error(FHIP_ERR_SHAPE, "%s: n_kv must be 1..=4096, got %zu", who, kv->n_kv);
+    if (kv->n_seq > 65535) return set_error(FHIP_ERR_SHAPE, "%s: more than 65535 sequences", who);
+    if (kv->n_pages > 0xFFFFFFFEull) return set_error(FHIP_ERR_SHAPE, "%s: more than 2^32 - 2 pages", who);
+    if (kv->pages_per_seq > 0xFFFFFFFFull / kv->page_rows) return set_error(FHIP_ERR_SHAPE, "%s: a sequence's rows reach 2^32", who);
+    if (kv->table_stride < kv->pages_per_seq) return set_error(FHIP_ERR_SHAPE, "%s: table_stride %zu is less than pages_per_seq %zu", who, kv->table_stride, kv->pages_per_seq);
+    if (!kv->d_k || !kv->d_v || !aligned16(kv->d_k) || !aligned16(kv->d_v)) return set_error(FHIP_ERR_ARG, "%s: the pools must be 16-byte aligned device memory", who);
+    if (kv->type == FHIP_Q8_0 && (!kv->d_k_scales || !kv->d_v_scales || !aligned16(kv->d_k_scales) || !aligned16(kv->d_v_scales)))
+        return set_error(FHIP_ERR_ARG, "%s: a Q8_0 cache has scales, 16-byte aligned", who);
+    if (!kv->d_table) return set_error(FHIP_ERR_ARG, "%s: NULL table", who);
+    v.k = kv->d_k; v.v = kv->d_v;
+    v.k_scales = (uint16_t*)kv->d_k_scales; v.v_scales = (uint16_t*)kv->d_v_scales;
+    v.table = kv->d_table; v.table_stride = kv->table_stride;
+    v.n_seq = (uint32_t)kv->n_seq; v.pages_per_seq = (uint32_t)kv->pages_per_seq; v.n_pages = (uint32_t)kv->n_pages;
+    v.n_kv = (int)kv->n_kv;
+    v.shift = __builtin_ctz(kv->page_rows);
+    return FHIP_OK;
+}
+static int paged_heads(const char* who, const fhip_paged* kv, size_t n_head) {
+    if (n_head < kv->n_kv || n_head % kv->n_kv != 0 || n_head / kv->n_kv > 16)
+        return set_error(FHIP_ERR_SHAPE, "%s: n_head must be a multiple of n_kv up to 16 times it, got %zu over %zu", who, n_head, kv->n_kv);
+    return FHIP_OK;
+}
+static uint32_t paged_bound(size_t n) { return n < 0xFFFFFFFFull ? (uint32_t)n : 0xFFFFFFFFu; }
+
+int fhip_paged_append(const fhip_paged* kv, const float* d_qkv, const float* d_bias, const float* d_q_norm, const float* d_k_norm, const uint32_t* d_seqs,
+                      const uint32_t* d_positions, const float* d_freq_scale, size_t t, size_t n_head, size_t n_rot, int interleaved, float eps, float base,
+                      float* d_q_out, void* stream) {
+    fhip::PagedView v;
+    int rc = paged_view("fhip_paged_append", kv, v);
+    if (rc || (rc = paged_heads("fhip_paged_append", kv, n_head)) || (rc = rope_checks("fhip_paged_append", n_head + 2 * kv->n_kv, kv->head_dim, n_rot))) return rc;
+    if (t == 0) return FHIP_OK;
+    if (t > 0x7FFFFFFFull) return set_error(FHIP_ERR_SHAPE, "fhip_paged_append: more than 2^31 - 1 tokens");
+    if (n_rot > 0 && !(base > 0.f)) return set_error(FHIP_ERR_ARG, "fhip_paged_append: base must be > 0");
+    if (!d_qkv || !d_positions || !d_q_out) return set_error(FHIP_ERR_ARG, "fhip_paged_append: NULL pointer");
+    if (!aligned16(d_qkv) || !aligned16(d_q_out) || !aligned16(d_bias) || !aligned16(d_q_norm) || !aligned16(d_k_norm))
+        return set_error(FHIP_ERR_ARG, "fhip_paged_append: pointers must be 16-byte aligned");
+    if ((rc = need_init())) return rc;
+    fhip::PagedPost p;
+    p.qkv = d_qkv; p.bias = d_bias; p.q_norm = d_q_norm; p.k_norm = d_k_norm; p.seqs = d_seqs; p.pos = d_positions; p.freq_scale = d_freq_scale; p.q_out = d_q_out;
+    p.t = (uint32_t)t; p.n_head = (int)n_head; p.n_rot = (int)n_rot; p.interleaved = interleaved != 0; p.eps = eps;
+    p.rate = n_rot > 0 ? -2.0 / (double)n_rot * log((double)base) : 0.0;
+    return fhip::launch_paged_append(kv->type, (int)kv->head_dim, v, p, (hipStream_t)stream);
+}
+
+size_t fhip_paged_attention_ws_bytes(const fhip_paged* kv, size_t n_head, size_t max_len) {
+    fhip::PagedView v;
+    if (paged_view("fhip_paged_attention_ws_bytes", kv, v) || paged_heads("fhip_paged_attention_ws_bytes", kv, n_head)) return 0;
+    return fhip::paged_attention_ws_bytes(v, (int)kv->head_dim, (int)n_head, paged_bound(max_len));
+}
+static int paged_attention(const char* who, const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, size_t max_len, const uint32_t* d_selected, size_t n_select,
+                           size_t n_head, size_t window, float softcap, float* d_ws, float* d_out, void* stream) {
+    fhip::PagedView v;
+    int rc = paged_view(who, kv, v);
+    if (rc || (rc = paged_heads(who, kv, n_head))) return rc;
+    if (!(softcap >= 0.f)) return set_error(FHIP_ERR_ARG, "%s: softcap must be >= 0", who);
+    if (kv->n_seq == 0) return FHIP_OK;
+    if (!d_q || !d_lens || !d_out) return set_error(FHIP_ERR_ARG, "%s: NULL pointer", who);
+    if (!aligned16(d_q) || !aligned16(d_out) || !aligned16(d_ws)) return set_error(FHIP_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
+    if ((rc = need_init())) return rc;
+    const uint32_t bound = paged_bound(max_len);
+    if (!d_ws && fhip::paged_attention_ws_bytes(v, (int)kv->head_dim, (int)n_head, d_selected ? paged_bound(n_select * kv->page_rows) : bound) > 0)
+        return set_error(FHIP_ERR_ARG, "%s: this call needs a workspace (fhip_paged_attention_ws_bytes)", who);
+    return fhip::launch_paged_attention(kv->type, (int)kv->head_dim, v, d_q, d_lens, bound, d_selected, (uint32_t)n_select, (int)n_head, paged_bound(window), softcap, d_ws,
+                                        d_out, (hipStream_t)stream);
+}
+int fhip_paged_attention(const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, size_t max_len, size_t n_head, size_t window, float softcap, float* d_ws,
+                         float* d_out, void* stream) {
+    return paged_attention("fhip_paged_attention", kv, d_q, d_lens, max_len, nullptr, 0, n_head, window, softcap, d_ws, d_out, stream);
+}
+static int select_count(const char* who, size_t n_select) {
+    if (n_select < 1 || n_select > (1u << 20)) return set_error(FHIP_ERR_SHAPE, "%s: n_select must be 1..=1048576, got %zu", who, n_select);
+    return FHIP_OK;
+}
+int fhip_paged_attention_selected(const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, const uint32_t* d_selected, size_t n_select, size_t n_head, float softcap,
+                                  float* d_ws, float* d_out, void* stream) {
+    if (!d_selected) return set_error(FHIP_ERR_ARG, "fhip_paged_attention_selected: NULL pointer");
+    int rc = select_count("fhip_paged_attention_selected", n_select);
+    if (rc) return rc;
+    return paged_attention("fhip_paged_attention_selected", kv, d_q, d_lens, 0xFFFFFFFFu, d_selected, n_select, n_head, 0, softcap, d_ws, d_out, stream);
+}
+
+int fhip_paged_key_bounds(const fhip_paged* kv, const uint32_t* d_lens, const uint32_t* d_new, size_t max_new, float* d_bounds, void* stream) {
+    fhip::PagedView v;
+    int rc = paged_view("fhip_paged_key_bounds", kv, v);
+    if (rc) return rc;
+    if (kv->n_seq == 0 || kv->pages_per_seq == 0 || max_new == 0) return FHIP_OK;
+    if (!d_lens || !d_bounds) return set_error(FHIP_ERR_ARG, "fhip_paged_key_bounds: NULL pointer");
+    if ((rc = need_init())) return rc;
+    return fhip::launch_paged_key_bounds(kv->type, (int)kv->head_dim, v, d_lens, d_new, paged_bound(max_new), d_bounds, (hipStream_t)stream);
+}
+
+size_t fhip_paged_select_ws_bytes(const fhip_paged* kv, size_t max_len) {
+    fhip::PagedView v;
+    if (paged_view("fhip_paged_select_ws_bytes", kv, v)) return 0;
+    return fhip::paged_select_ws_bytes(v, paged_bound(max_len));
+}
+int fhip_paged_select(const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, size_t max_len, const float* d_bounds, size_t n_head, size_t n_select,
+                      size_t keep_first, size_t keep_last, void* d_ws, uint32_t* d_selected, void* stream) {
+    fhip::PagedView v;
+    int rc = paged_view("fhip_paged_select", kv, v);
+    if (rc || (rc = paged_heads("fhip_paged_select", kv, n_head)) || (rc = select_count("fhip_paged_select", n_select))) return rc;
+    if (keep_first > n_select || keep_last > n_select - keep_first)
+        return set_error(FHIP_ERR_SHAPE, "fhip_paged_select: keep_first %zu and keep_last %zu exceed n_select %zu", keep_first, keep_last, n_select);
+    if (kv->n_seq == 0) return FHIP_OK;
+    const uint32_t bound = paged_bound(max_len);
+    if (!d_q || !d_lens || !d_bounds || !d_selected || (!d_ws && fhip::paged_select_ws_bytes(v, bound) > 0)) return set_error(FHIP_ERR_ARG, "fhip_paged_select: NULL pointer");
+    if (!aligned16(d_q) || !aligned16(d_bounds) || !aligned16(d_ws)) return set_error(FHIP_ERR_ARG, "fhip_paged_select: pointers must be 16-byte aligned");
+    if ((rc = need_init())) return rc;
+    return fhip::launch_paged_select((int)kv->head_dim, v, d_q, d_lens, bound, d_bounds, (int)n_head, (uint32_t)n_select, (uint32_t)keep_first, (uint32_t)keep_last, d_ws,
+                                     d_selected, (hipStream_t)stream);
+}
+
+int fhip_paged_rows(const fhip_paged* kv, size_t seq, size_t row0, size_t rows, float* d_k_out, float* d_v_out, void* stream) {
+    fhip::PagedView v;
+    int rc = paged_view("fhip_paged_rows", kv, v);
+    if (rc) return rc;
+    const size_t cap = kv->pages_per_seq * kv->page_rows;
+    if (seq >= kv->n_seq) return set_error(FHIP_ERR_SHAPE, "fhip_paged_rows: sequence %zu of %zu", seq, kv->n_seq);
+    if (row0 > cap || rows > cap - row0) return set_error(FHIP_ERR_SHAPE, "fhip_paged_rows: rows %zu + %zu past the %zu that the table reaches", row0, rows, cap);
+    if (rows == 0) return FHIP_OK;
+    if (!d_k_out || !d_v_out || !aligned16(d_k_out) || !aligned16(d_v_out)) return set_error(FHIP_ERR_ARG, "fhip_paged_rows: outputs must be 16-byte aligned device memory");
+    if ((rc = need_init())) return rc;
+    return fhip::launch_paged_rows(kv->type, (int)kv->head_dim, v, (uint32_t)seq, row0, rows, d_k_out, d_v_out, (hipStream_t)stream);
 }
 
 }  // extern "C"

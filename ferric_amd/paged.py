@@ -1,0 +1,147 @@
+"""A paged key/value cache: the keys and values of many sequences in one pool of pages that a table names, and what fills and reads it.
+
+For a server that decodes sequences of different lengths together: `append` post-processes and stores new tokens' rows, `attention` is one new token
+of every sequence over all of its rows (or a window), `key_bounds` / `select` / `attention_selected` the same over the pages whose
+keys promise most, `rows` a cached prefix as f32 rows for decode.causal_attention. The reference keeps one sequence a cache and has no
+counterpart. Everything runs through libferric_hip; there is no CPU path.
+"""
+import ctypes as C
+
+import numpy as np
+
+from . import _lib
+from .qmatrix import BF16, F16, F32, Q8_0, DeviceBuffer, Tensor, _arrived, _stream_handle, _upload
+
+ALL = (F32, F16, BF16, Q8_0)
+NO_PAGE = 0xFFFFFFFF
+_VALUE_BYTES = {F32: 4, F16: 2, BF16: 2, Q8_0: 1}
+
+
+def _ptr(t):
+    return None if t is None else t.buf.ptr
+
+
+class PagedKvCache:
+    """Pools [n_pages * page_rows, n_kv * head_dim] of keys and of values (type F32, F16, BF16 or Q8_0: codes and f16 scales as kvquant stores them) and a table
+    [n_seq, pages_per_seq] of page numbers: position p of sequence i is row table[i, p / page_rows] * page_rows + p % page_rows. Which page belongs to whom is
+    the caller's to decide (set_table)."""
+
+    def __init__(self, ty, page_rows, n_pages, n_kv, head_dim, n_seq, pages_per_seq):
+        assert ty in ALL, f"a paged cache holds F32, F16, BF16 or Q8_0, not ggml type {ty}"
+        values = n_pages * page_rows * n_kv * head_dim
+        pools = [DeviceBuffer(max(values * _VALUE_BYTES[ty], 16)) for _ in range(2)]
+        scales = [DeviceBuffer(max(values // 32 * 2, 16)) if ty == Q8_0 else None for _ in range(2)]
+        table = DeviceBuffer(max(4 * n_seq * pages_per_seq, 16))
+        self._take(ty, page_rows, n_pages, n_kv, head_dim, *pools, *scales, table, n_seq, pages_per_seq)
+        self.set_table(np.full((n_seq, pages_per_seq), NO_PAGE, np.uint32))
+
+    @staticmethod
+    def wrap(ty, page_rows, n_pages, n_kv, head_dim, k, v, k_scales, v_scales, table, n_seq, pages_per_seq):
+        """Over device memory the caller already has (objects with a `ptr`, kept alive here); scales None unless Q8_0."""
+        cache = object.__new__(PagedKvCache)
+        cache._take(ty, page_rows, n_pages, n_kv, head_dim, k, v, k_scales, v_scales, table, n_seq, pages_per_seq)
+        return cache
+
+    def _take(self, ty, page_rows, n_pages, n_kv, head_dim, k, v, k_scales, v_scales, table, n_seq, pages_per_seq):
+        _lib.init()
+        self.type, self.page_rows, self.n_pages, self.n_kv, self.head_dim = ty, page_rows, n_pages, n_kv, head_dim
+        self.k, self.v, self.k_scales, self.v_scales, self.table, self.n_seq, self.pages_per_seq = k, v, k_scales, v_scales, table, n_seq, pages_per_seq
+        at = lambda b: None if b is None else getattr(b.ptr, "value", b.ptr)      # noqa: E731
+        self._desc = _lib.Paged(ty, page_rows, n_pages, n_kv, head_dim, at(k), at(v), at(k_scales), at(v_scales), at(table), n_seq, pages_per_seq, pages_per_seq)
+        self._ref = C.byref(self._desc)
+        self._ws = {}
+
+    def set_table(self, pages, stream=None):
+        """The whole table from the host, [n_seq, pages_per_seq]; NO_PAGE (or any number past the pool) where a sequence has none."""
+        a = np.ascontiguousarray(pages, dtype=np.uint32)
+        assert a.shape == (self.n_seq, self.pages_per_seq), f"the table is {[self.n_seq, self.pages_per_seq]}, not {list(a.shape)}"
+        if a.nbytes:
+            _upload(self.table, a, stream)
+            _arrived(a, stream)
+
+    def _workspace(self, need, ws, stream):
+        """The caller's, or one kept for the stream. What was outgrown stays: a graph captured on the stream may name it. Graphs that may run at the same time need
+        workspaces of their own."""
+        if ws is not None or need == 0:
+            return None if ws is None else ws.ptr
+        kept = self._ws.setdefault(None if stream is None else stream.handle.value, [])
+        if not kept or kept[-1].nbytes < need:
+            kept.append(DeviceBuffer(1 << (need - 1).bit_length()))
+        return kept[-1].ptr
+
+    def append(self, qkv, seqs, positions, n_heads, base, n_rot=None, interleaved=False, eps=1e-6, bias=None, q_norm=None, k_norm=None, freq_scale=None, out=None, stream=None):
+        """Post-processes the fused rows qkv [t, (n_heads + 2 n_kv) * head_dim] of t new tokens (bias, head norm, rotation), stores their keys and values, returns their
+        queries [t, n_heads * head_dim]. seqs, positions: device u32 Tensors [t]; seqs None: token i is of sequence i."""
+        t, width = qkv.shape
+        assert width == (n_heads + 2 * self.n_kv) * self.head_dim, f"append: rows of {width} values are not {n_heads} + 2 * {self.n_kv} heads of {self.head_dim}"
+        assert positions.numel() == t and (seqs is None or seqs.numel() == t), "append: one position and one sequence a row"
+        assert (bias is None or bias.numel() == width) and all(w is None or w.numel() == self.head_dim for w in (q_norm, k_norm)), "append: bias or norm of another size"
+        n_rot = self.head_dim if n_rot is None else n_rot
+        assert freq_scale is None or 2 * freq_scale.numel() >= n_rot, "append: a frequency scale for every pair"
+        assert seqs is not None or t <= self.n_seq, "append: more rows than sequences"
+        q = Tensor.empty((t, n_heads * self.head_dim)) if out is None else out
+        assert q.shape == (t, n_heads * self.head_dim), "append: out has another shape"
+        _lib.check(_lib.load().fhip_paged_append(self._ref, qkv.buf.ptr, _ptr(bias), _ptr(q_norm), _ptr(k_norm), _ptr(seqs), positions.buf.ptr, _ptr(freq_scale), t, n_heads, n_rot,
+                                                 int(interleaved), eps, base, q.buf.ptr, _stream_handle(stream)))
+        return q
+
+    def _query(self, q, lens, n_heads, out):
+        assert q.shape == (self.n_seq, n_heads * self.head_dim), f"one query row a sequence: {[self.n_seq, n_heads * self.head_dim]}, not {list(q.shape)}"
+        assert lens.numel() == self.n_seq, "one length a sequence"
+        if out is None:
+            return Tensor.empty(q.shape)
+        assert out.shape == q.shape, "out has another shape"
+        return out
+
+    def attention(self, q, lens, max_len, n_heads, window=0, softcap=0.0, out=None, ws=None, stream=None):
+        """One new token of every sequence, q [n_seq, n_heads * head_dim], over the first lens[i] rows (device u32 Tensor, the new token's own among them; at most
+        max_len) or the newest `window` of them."""
+        out = self._query(q, lens, n_heads, out)
+        lib = _lib.load()
+        need = lib.fhip_paged_attention_ws_bytes(self._ref, n_heads, max_len)
+        _lib.check(lib.fhip_paged_attention(self._ref, q.buf.ptr, lens.buf.ptr, max_len, n_heads, window, softcap, self._workspace(need, ws, stream), out.buf.ptr,
+                                            _stream_handle(stream)))
+        return out
+
+    def empty_bounds(self):
+        """Room for the pages' key bounds, [n_pages, n_kv, 2, head_dim]; key_bounds fills a page's when its first row is appended."""
+        return Tensor.empty((self.n_pages, self.n_kv, 2, self.head_dim))
+
+    def key_bounds(self, lens, max_new, bounds, fresh=None, stream=None):
+        """Takes the keys of each sequence's last `fresh` rows (device u32 Tensor; None: max_new) into their pages' bounds, in place."""
+        assert lens.numel() == self.n_seq and (fresh is None or fresh.numel() == self.n_seq), "one length a sequence"
+        assert bounds.numel() == self.n_pages * self.n_kv * 2 * self.head_dim, "key_bounds: bounds of another size"
+        _lib.check(_lib.load().fhip_paged_key_bounds(self._ref, lens.buf.ptr, _ptr(fresh), max_new, bounds.buf.ptr, _stream_handle(stream)))
+        return bounds
+
+    def select(self, q, lens, max_len, bounds, n_heads, n_select, first=1, last=1, out=None, ws=None, stream=None):
+        """The n_select pages of every sequence and KV head that promise most, [n_seq, n_kv, n_select] u32, ascending, NO_PAGE behind the last."""
+        self._query(q, lens, n_heads, q)
+        assert bounds.numel() == self.n_pages * self.n_kv * 2 * self.head_dim, "select: bounds of another size"
+        shape = (self.n_seq, self.n_kv, n_select)
+        out = Tensor.empty(shape, np.uint32) if out is None else out
+        assert out.shape == shape, "select: out has another shape"
+        lib = _lib.load()
+        need = lib.fhip_paged_select_ws_bytes(self._ref, max_len)
+        _lib.check(lib.fhip_paged_select(self._ref, q.buf.ptr, lens.buf.ptr, max_len, bounds.buf.ptr, n_heads, n_select, first, last, self._workspace(need, ws, stream), out.buf.ptr,
+                                         _stream_handle(stream)))
+        return out
+
+    def attention_selected(self, q, lens, selected, n_heads, softcap=0.0, out=None, ws=None, stream=None):
+        """attention over the rows of the selected pages [n_seq, n_kv, n] only."""
+        out = self._query(q, lens, n_heads, out)
+        assert selected.shape[:2] == (self.n_seq, self.n_kv) and len(selected.shape) == 3, "selected is [n_seq, n_kv, n]"
+        n = selected.shape[2]
+        lib = _lib.load()
+        need = lib.fhip_paged_attention_ws_bytes(self._ref, n_heads, n * self.page_rows)
+        _lib.check(lib.fhip_paged_attention_selected(self._ref, q.buf.ptr, lens.buf.ptr, selected.buf.ptr, n, n_heads, softcap, self._workspace(need, ws, stream), out.buf.ptr,
+                                                     _stream_handle(stream)))
+        return out
+
+    def rows(self, seq, row0, rows, out=None, stream=None):
+        """Rows row0 .. row0 + rows of sequence seq as f32: (k, v), [rows, n_kv * head_dim] each."""
+        shape = (rows, self.n_kv * self.head_dim)
+        k, v = (Tensor.empty(shape), Tensor.empty(shape)) if out is None else out
+        assert k.shape == v.shape == shape, "rows: out has another shape"
+        _lib.check(_lib.load().fhip_paged_rows(self._ref, seq, row0, rows, k.buf.ptr, v.buf.ptr, _stream_handle(stream)))
+        return k, v

@@ -439,6 +439,62 @@ int fhip_qkv_post_attention_kvq(int fmt, const float* d_qkv, const float* d_bias
                                 float base, uint32_t* d_k_codes, uint32_t* d_k_scales, uint32_t* d_v_codes, uint32_t* d_v_scales, size_t cap, size_t len,
                                 size_t window, float softcap, float* d_ws, float* d_out, void* stream);
 
+/* ---- a paged key/value cache: many sequences in one pool of pages, for a server that decodes them together. The reference keeps one sequence a cache
+ * (crates/ferric-tensor/src/lib.rs:1287 KvBuf) and has no counterpart. ---- */
+
+/* A description the caller owns; it is read during the call, the device memory it names later, by the work that the call enqueues. A pool row holds one token's n_kv * head_dim
+ * values; position p of sequence i is row table[i * table_stride + p / page_rows] * page_rows + p % page_rows of the pools. Several sequences may name one page
+ * (a common prefix). A table entry that is no page of the pool (n_pages and more) has no rows: what would be stored there is dropped, what would be read is left out.
+ * Checked by every call below: type one of FHIP_F32, FHIP_F16, FHIP_BF16, FHIP_Q8_0 (FHIP_ERR_UNSUPPORTED_TYPE); head_dim 64 or 128; page_rows a power of two from 16 to 4096;
+ * n_kv from 1 to 4096; n_seq up to 65535; up to 2^32 - 2 pages, a sequence's rows below 2^32; table_stride at least pages_per_seq (FHIP_ERR_SHAPE); pools 16-byte aligned, scales not NULL for Q8_0 (FHIP_ERR_ARG). */
+typedef struct fhip_paged {
+    uint32_t type;            /* what the pools hold */
+    uint32_t page_rows;
+    size_t n_pages, n_kv, head_dim;
+    void *d_k, *d_v;          /* [n_pages * page_rows, n_kv * head_dim] values; Q8_0: int8 codes, the code words of fhip_kvq_append */
+    void *d_k_scales, *d_v_scales; /* Q8_0: an f16 scale for each 32 values, the scale words of fhip_kvq_append; otherwise not looked at */
+    const uint32_t* d_table;  /* [n_seq, table_stride] */
+    size_t n_seq, pages_per_seq, table_stride; /* pages_per_seq: entries of a row of the table that may be read */
+} fhip_paged;
+
+/* fhip_qkv_post on a paged cache, for t new tokens of any of its sequences: bias, per-head RMSNorm, rotary embedding, query heads to d_q_out [t, n_head * head_dim], key and value
+ * heads rounded once (to nearest, ties to even; Q8_0 as fhip_kvq_append rounds) to their row. Token i is row d_positions[i] of sequence d_seqs[i] (NULL: of sequence i); one that the
+ * table or d_seqs has no place for leaves its query only. No two tokens of a call may have the same place. n_head is a multiple of n_kv, up to 16 times it.
+ * The angle position * base^(-2c / n_rot) [* d_freq_scale[c]] is formed in f64 (fhip_qkv_post rounds the frequency and the product to f32, 4e-3 rad at position 100 000), so rows differ
+ * from its rows by that. A token's row has the same bits in every batch. Pointers 16-byte aligned; d_q_out may not overlap d_qkv. t = 0: nothing is done. */
+int fhip_paged_append(const fhip_paged* kv, const float* d_qkv, const float* d_bias, const float* d_q_norm, const float* d_k_norm, const uint32_t* d_seqs,
+                      const uint32_t* d_positions, const float* d_freq_scale, size_t t, size_t n_head, size_t n_rot, int interleaved, float eps, float base,
+                      float* d_q_out, void* stream);
+
+/* One new token of every sequence: q [n_seq, n_head * head_dim] against the first d_lens[i] rows of sequence i (the token's own among them), or the newest `window` of these when
+ * window > 0; softcap as fhip_decode_attention_ex. out[i, h] = softmax_j(q . K_j / sqrt(head_dim)) @ V, query head h with KV head h / (n_head / n_kv), n_head a multiple of n_kv up to
+ * 16 times it. d_lens is read on the device, so one captured launch serves growing sequences; max_len is the host's bound that sizes the work: a longer length is cut
+ * to it and to what the table reaches. A length of 0, or no row left, gives zeros. f32 arithmetic, the rows enter as the values they stand for; the same inputs give the same bits. What lies
+ * behind a sequence's last row is never part of a result, whatever it holds. d_ws: fhip_paged_attention_ws_bytes(kv, n_head, max_len) bytes of scratch, 16-byte aligned (NULL when
+ * that is 0), the call's own until the stream has passed it. */
+size_t fhip_paged_attention_ws_bytes(const fhip_paged* kv, size_t n_head, size_t max_len);
+int fhip_paged_attention(const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, size_t max_len, size_t n_head, size_t window, float softcap, float* d_ws,
+                         float* d_out, void* stream);
+
+/* Sparse attention over the pages whose keys promise most. d_bounds [n_pages, n_kv, 2, head_dim]: smallest and largest value of each dim among a page's keys, kept up to date
+ * by the caller's calls of fhip_paged_key_bounds behind its appends: the last d_new[i] rows of sequence i (NULL: max_new; never more than max_new or d_lens[i]) are new, a page whose first row
+ * is new starts over, the others' bounds widen. No two sequences may have new rows in one page. NaN keys make NaN bounds. */
+int fhip_paged_key_bounds(const fhip_paged* kv, const uint32_t* d_lens, const uint32_t* d_new, size_t max_new, float* d_bounds, void* stream);
+/* d_selected [n_seq, n_kv, n_select]: for each sequence and KV head the first keep_first and last keep_last of its pages, then those of the highest score, the largest q . k that a key
+ * within the bounds can have for any of the head's queries (formed in f64; equal ones by their place, a NaN first); as ascending indices into the sequence's row of the table, filled up with 0xFFFFFFFF.
+ * n_select at least keep_first + keep_last and 1, at most 2^20 (FHIP_ERR_SHAPE). d_ws: fhip_paged_select_ws_bytes(kv, max_len) bytes, 16-byte aligned. */
+size_t fhip_paged_select_ws_bytes(const fhip_paged* kv, size_t max_len);
+int fhip_paged_select(const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, size_t max_len, const float* d_bounds, size_t n_head, size_t n_select,
+                      size_t keep_first, size_t keep_last, void* d_ws, uint32_t* d_selected, void* stream);
+/* fhip_paged_attention over the rows of the listed pages only (an index that is no page of the sequence's d_lens[i] rows is left out, each may be listed once). d_ws:
+ * fhip_paged_attention_ws_bytes(kv, n_head, n_select * page_rows) bytes. */
+int fhip_paged_attention_selected(const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, const uint32_t* d_selected, size_t n_select, size_t n_head, float softcap,
+                                  float* d_ws, float* d_out, void* stream);
+
+/* Rows row0 .. row0 + rows - 1 of one sequence as f32, K to d_k_out and V to d_v_out [rows, n_kv * head_dim], 16-byte aligned: a cached prefix for fhip_causal_attention
+ * over a prompt's next block. seq >= n_seq or rows past pages_per_seq pages: FHIP_ERR_SHAPE; rows of an entry that is no page of the pool are left as they were. */
+int fhip_paged_rows(const fhip_paged* kv, size_t seq, size_t row0, size_t rows, float* d_k_out, float* d_v_out, void* stream);
+
 /* rmsnorm / add_rmsnorm (lib.rs:346, :372) fused into the mat-vec that consumes it, for ONE activation row:
  *   h = rmsnorm(x [+ resid], norm_w, eps);   y = h W^T   (swiglu != 0: y = silu(gate . h) * (up . h), as fhip_matmul_q_swiglu)
  * and, when d_x_out is given, x_out = x + resid (the next residual). Neither x_out nor y may overlap x, resid, norm_w or each

@@ -383,105 +383,570 @@ __global__ __launch_bounds__(SEL_T) void select_kernel(PagedView kv, const uint3
 }
 
 // ---------------------------------------------------------------- attention of one token of every sequence
-// out[h] = sum_j softmax_j(q_h . K_j / sqrt(hd)) V_j over the rows of the sequence, the g query heads of a KV head together, on v_mfma_f32_16x16x4_f32: products of f32
-// operands and sums in f32, whatever the rows are stored in. A wave takes 16 keys at a time. K q^T puts head n in lane n's column and keys 4 (lane / 16) + r in its four
-// registers, which is where V^T p^T wants its second operand's four keys, one per instruction: nothing is exchanged between the products, and a head's running
-// maximum and sum stay in its column's lanes. Lane (m, k = lane / 16) of the first operand holds four neighbouring dims of key m, or four of key 4 k + r for V: both products are
-// indifferent to which dims an instruction takes as long as both operands agree, so all loads are of 16 neighbouring bytes.
-// SEL: the rows of the listed pages instead of all.
-constexpr int ATT_W = 4;
-template <int TYPE, int HD, bool SEL>
-__global__ __launch_bounds__(64 * ATT_W) void attention_kernel(PagedView kv, const float* __restrict__ q, const uint32_t* __restrict__ lens, uint32_t max_len,
-                                                               const uint32_t* __restrict__ selected, uint32_t n_select, int n_head, uint32_t window, float softcap, float scale,
-                                                               float* __restrict__ out) {
-    constexpr int NI = HD / 16;
-    __shared__ float sm_m[ATT_W][16], sm_l[ATT_W][16];
-    __shared__ __attribute__((aligned(16))) float sm_o[ATT_W][16][HD + 4];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kg = lane >> 4;
-    const int g = n_head / kv.n_kv, head = blockIdx.x % kv.n_kv;
-    const uint32_t seq = blockIdx.x / kv.n_kv, R = 1u << kv.shift;
-    const uint32_t len = rows_of(kv, lens, seq, max_len), lo = window && window < len ? len - window : 0;
-    const uint32_t* table = kv.table + seq * kv.table_stride;
-    const uint32_t* list = SEL ? selected + (size_t)blockIdx.x * n_select : nullptr;
-    f32x4 qf[NI];
-    const float* qh = q + ((size_t)seq * n_head + head * g + (n < g ? n : 0)) * HD;
+// out[h] = sum_j softmax_j(q_h . K_j / sqrt(hd)) V_j over the rows of the sequence, the g <= 16 query heads of a KV head together on the matrix cores, f32 grade whatever the rows
+// are stored in. A wave takes a step of 16 keys (f32) or 32 (two tiles of 16, the other types) at a time.
+//
+// K q^T puts head n in lane n's column and keys 4 (lane / 16) + r of a tile in its four registers, which is where V^T p^T wants its second operand's keys: nothing is exchanged
+// between the two products, and a head's running maximum and sum stay in its column's lanes. Both products are indifferent to which dims or keys share an instruction as
+// long as their operands agree, so a lane's loads are of neighbouring bytes of one row: of a key's dims for K, of eight keys' same dims for V.
+//   f32    v_mfma_f32_16x16x4_f32 on the rows as they are.
+//   bf16   v_mfma_f32_16x16x32_bf16; q and p as three bf16 values each, cut off rather than rounded, so that they add up to the f32 value.
+//   f16    v_mfma_f32_16x16x32_f16; q (times a power of two that brings its largest value to 2^14) and p (times 2^15) as two f16 values, 22 bits.
+//   Q8_0   keys as f16 holds their codes, q as for f16, a block of 32 dims an instruction, whose sum is multiplied by the block's scale; values as c * d on the f32 instruction.
+// Bound by the rows' bytes. The next step's keys are requested once the current ones are multiplied, its values once the current ones are: eight waves a CU keep 64 KB and more
+// on the way without a second set of registers.
+//
+// Work is dealt out by the device, as only it knows the lengths: the steps of all (sequence, KV head) units in a row are cut into equal ranges, a workgroup each, whatever the
+// lengths are. A unit that lies within one range is finished there; of others every workgroup leaves (maximum, sum, weighted rows) in the workspace and join_kernel adds them in order.
+// SEL: the steps are those of the listed pages.
+constexpr float LOG2E = 1.4426950408889634f;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+union Frag {
+    uint32_t w[4];
+    bf16x8 b;
+    f16x8 h;
+};
+// the upper halves of two words, the first one's in the lower half
+__device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ uint32_t lower_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+// Two f32 as PARTS 16-bit values each: word i of the result holds part i of both.
+template <bool BF>
+__device__ __forceinline__ void cut(float a, float b, uint32_t (&w)[3]) {
+    if constexpr (BF) {
 #pragma unroll
-    for (int i = 0; i < NI; i++) {
-        qf[i] = *(const f32x4*)(qh + 16 * i + 4 * kg);
-        if (n >= g) qf[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 3; i++) {
+            w[i] = upper_halves(__float_as_uint(a), __float_as_uint(b));
+            a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+            b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+        }
+    } else {
+        const f16x2 hi = __builtin_bit_cast(f16x2, pack_f16(a, b));
+        w[0] = __builtin_bit_cast(uint32_t, hi);
+        w[1] = pack_f16(a - (float)hi.x, b - (float)hi.y);
     }
-    f32x4 acc[NI];                                    // acc[4 h + c][r]: dim 64 h + 4 (4 kg + r) + c of head n
+}
+
+template <int TYPE>
+struct Path {
+    static constexpr int TILES = TYPE == FHIP_F32 ? 1 : 2;            // of 16 keys a step
+    static constexpr int KEYS = 16 * TILES;
+    static constexpr int PARTS = TYPE == FHIP_BF16 ? 3 : 2;
+    static constexpr bool HALF = TYPE != FHIP_F32;                    // K on a 16-bit instruction
+    static constexpr bool HALF_V = TYPE == FHIP_BF16 || TYPE == FHIP_F16;
+};
+
+// Keys of sequence `seq` that are attended to, [lo, len), and the steps that they lie in.
+struct Span {
+    uint32_t len, lo, first, steps;
+};
+template <int TYPE, bool SEL>
+__device__ __forceinline__ Span span_of(const PagedView& kv, const uint32_t* __restrict__ lens, uint32_t seq, uint32_t max_len, uint32_t window, uint32_t n_select) {
+    constexpr int KEYS = Path<TYPE>::KEYS;
+    Span s;
+    s.len = kv.n_pages ? rows_of(kv, lens, seq, max_len) : 0;
+    s.lo = window && window < s.len ? s.len - window : 0;
+    if constexpr (SEL) {
+        const uint32_t pages = pages_of(kv, s.len), listed = pages < n_select ? pages : n_select;
+        s.first = 0;
+        s.steps = (uint32_t)((((uint64_t)listed << kv.shift) + KEYS - 1) / KEYS);
+    } else {
+        s.first = s.lo / KEYS;
+        s.steps = s.len ? (s.len - 1) / KEYS + 1 - s.first : 0;
+    }
+    return s;
+}
+// Steps in front of sequence 64 b + lane in blocks of 64 sequences, and of all: a wave's scan.
+__device__ __forceinline__ uint64_t wave_scan(uint64_t v, int lane) {      // inclusive
 #pragma unroll
-    for (int i = 0; i < NI; i++) acc[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    const uint32_t first = SEL ? 0 : lo >> 4, tiles = SEL ? n_select << (kv.shift - 4) : (len + 15) >> 4;
-    for (uint32_t t = first + wave; t < tiles; t += ATT_W) {
-        const uint32_t entry = SEL ? list[t >> (kv.shift - 4)] : t >> (kv.shift - 4);
-        const uint32_t start = SEL ? (t & ((R >> 4) - 1)) << 4 : (t << 4) & (R - 1);        // of the tile in its page
-        if (SEL && entry >= pages_of(kv, len)) continue;
-        const uint32_t page = table[entry], pos = (entry << kv.shift) + start;
-        if (page >= kv.n_pages || (SEL && pos >= len)) continue;
-        const size_t row = ((size_t)page << kv.shift) + start;
-        f32x4 s = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const f32x4 k = load4<TYPE>(kv.k, kv.k_scales, ((row + n) * kv.n_kv + head) * HD + 16 * i + 4 * kg);
-#pragma unroll
-            for (int e = 0; e < 4; e++) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], qf[i][e], s, 0, 0, 0);
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t t = __shfl_up((unsigned long long)v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+
+struct Attend {
+    PagedView kv;
+    const float* q;
+    const uint32_t* lens;
+    const uint32_t* selected;
+    float *out, *part;      // part: per workgroup two times g rows of HD, then g (maximum, sum), and 2 g words to keep the next one aligned
+    uint32_t max_len, n_select, window;
+    int n_head;
+    float softcap, scale;
+    int log_wgs;            // the steps are dealt out to 1 << log_wgs workgroups, MIN_STEPS each at least; < 0: workgroup u has unit u
+    uint32_t min_steps;
+};
+
+// Range of steps of a workgroup: all steps over the workgroups, `least` at least.
+__device__ __forceinline__ uint64_t steps_each(uint64_t all, int log_wgs, uint32_t least) {
+    const uint64_t per = (all + ((uint64_t)1 << log_wgs) - 1) >> log_wgs;
+    return per > least ? per : least;
+}
+template <int TYPE, bool SEL>
+__device__ __forceinline__ uint64_t all_steps(const Attend& a, int lane) {
+    uint64_t all = 0;
+    for (uint32_t b = 0; b < a.kv.n_seq; b += 64) {
+        const uint64_t c = b + lane < a.kv.n_seq ? (uint64_t)span_of<TYPE, SEL>(a.kv, a.lens, b + lane, a.max_len, a.window, a.n_select).steps * a.kv.n_kv : 0;
+        all += __shfl((unsigned long long)wave_scan(c, lane), 63);
+    }
+    return all;
+}
+
+template <int TYPE, int HD, bool SEL, int WV>
+__global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
+    typedef Path<TYPE> P;
+    constexpr int TILES = P::TILES, PARTS = P::PARTS, NB = HD / 32, NJ = HD / 16;
+    constexpr int IDS = 64 / TILES;                   // steps whose pages a wave looks up at once
+    __shared__ float sm_m[WV][16], sm_l[WV][16];
+    __shared__ __attribute__((aligned(16))) float sm_o[WV][16][HD + 4];
+    const PagedView& kv = a.kv;
+    const int lane = threadIdx.x & 63, wave = WV == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, kg = lane >> 4;
+    const int g = a.n_head / kv.n_kv;
+
+    // this workgroup's steps, and the unit that the first of them belongs to
+    uint64_t at = 0, end = ~0ull, unit0 = 0;          // unit0: the first step of sequence `seq`
+    uint32_t seq = 0, head = 0, from = 0;
+    Span sp;
+    if (a.log_wgs < 0) {
+        seq = blockIdx.x / kv.n_kv;
+        head = blockIdx.x % kv.n_kv;
+        sp = span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select);
+    } else {
+        const uint64_t all = all_steps<TYPE, SEL>(a, lane), per = steps_each(all, a.log_wgs, a.min_steps);
+        at = blockIdx.x * per;
+        end = at + per < all ? at + per : all;
+        if (at >= end) return;
+        uint64_t before = 0;
+        for (uint32_t b = 0; b < kv.n_seq; b += 64) {
+            const uint64_t c = b + lane < kv.n_seq ? (uint64_t)span_of<TYPE, SEL>(kv, a.lens, b + lane, a.max_len, a.window, a.n_select).steps * kv.n_kv : 0;
+            const uint64_t upto = before + wave_scan(c, lane), here = __ballot(upto > at);
+            if (here) {
+                const int l = __builtin_ctzll(here);
+                seq = b + l;
+                unit0 = __shfl((unsigned long long)(upto - c), l);
+                break;
+            }
+            before = __shfl((unsigned long long)upto, 63);
         }
-        float top = m;
+        seq = __builtin_amdgcn_readfirstlane(seq);
+        sp = span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select);
+        head = (uint32_t)((at - unit0) / sp.steps);
+        from = (uint32_t)((at - unit0) - (uint64_t)head * sp.steps);
+    }
+    const uint64_t range0 = at;
+
+    for (;;) {
+        head = __builtin_amdgcn_readfirstlane(head);
+        const uint32_t to = a.log_wgs < 0 || end - at > sp.steps - from ? sp.steps : from + (uint32_t)(end - at);   // steps [from, to) of the unit
+        const uint32_t* table = kv.table + seq * kv.table_stride;
+        const uint32_t* list = SEL ? a.selected + ((size_t)seq * kv.n_kv + head) * a.n_select : nullptr;
+        const uint32_t pages = pages_of(kv, sp.len);
+
+        // the unit's queries, as the second operand of K q^T
+        float m = -INFINITY, l = 0.f, c2 = a.scale * (a.softcap > 0.f ? 1.f : LOG2E);
+        f32x4 qf[P::HALF ? 1 : NJ];
+        Frag qp[P::HALF ? NB : 1][P::HALF ? PARTS : 1];
+        {
+            const float* qh = a.q + ((size_t)seq * a.n_head + head * g + (n < g ? n : 0)) * HD;
+            if constexpr (!P::HALF) {
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            float x = s[r] * scale;
-            if (softcap > 0.f) x = softcap * tanhf(x / softcap);
-            const uint32_t at = pos + 4 * kg + r;
-            s[r] = at < len && at >= lo ? x : -INFINITY;
-            top = fmaxf(top, s[r]);
-        }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float base = top == -INFINITY ? 0.f : top, f = expf(m - base);
-        float p[4];
-        l *= f;
+                for (int i = 0; i < NJ; i++) {
+                    qf[i] = *(const f32x4*)(qh + 16 * i + 4 * kg);
+                    if (n >= g) qf[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                }
+            } else {
+                f32x4 raw[NB][2];
+                float top = 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            p[r] = expf(s[r] - base);
-            l += p[r];
-        }
-        m = top;
+                for (int i = 0; i < NB; i++)
 #pragma unroll
-        for (int i = 0; i < NI; i++) acc[i] *= f;
+                    for (int e = 0; e < 2; e++) {
+                        raw[i][e] = *(const f32x4*)(qh + 32 * i + 8 * kg + 4 * e);
+                        if (n >= g) raw[i][e] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const uint32_t at = pos + 4 * kg + r;
+                        for (int x = 0; x < 4; x++) top = fmaxf(top, fabsf(raw[i][e][x]));
+                    }
+                float up = 1.f;
+                if constexpr (TYPE != FHIP_BF16) {     // the head's largest |q| to [2^14, 2^15)
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const int ex = top > 0.f && top < INFINITY ? 14 - (int)(((__float_as_uint(top) >> 23) & 255u) - 127u) : 0;
+                    const int clipped = ex < -126 ? -126 : ex > 126 ? 126 : ex;
+                    up = __uint_as_float((uint32_t)(127 + clipped) << 23);
+                    c2 *= __uint_as_float((uint32_t)(127 - clipped) << 23);
+                }
 #pragma unroll
-            for (int h = 0; h < HD / 64; h++) {
-                f32x4 v = load4<TYPE>(kv.v, kv.v_scales, ((row + 4 * kg + r) * kv.n_kv + head) * HD + 64 * h + 4 * n);
-                if (!(at < len && at >= lo)) v = (f32x4){0.f, 0.f, 0.f, 0.f};      // what lies behind the last row is no number, maybe
+                for (int i = 0; i < NB; i++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) acc[4 * h + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[c], p[r], acc[4 * h + c], 0, 0, 0);
+                    for (int x = 0; x < 4; x++) {
+                        uint32_t w[3];
+                        cut<TYPE == FHIP_BF16>(raw[i][x / 2][2 * (x & 1)] * up, raw[i][x / 2][2 * (x & 1) + 1] * up, w);
+#pragma unroll
+                        for (int p = 0; p < PARTS; p++) qp[i][p].w[x] = w[p];
+                    }
             }
         }
-    }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    if (kg == 0) { sm_m[wave][n] = m; sm_l[wave][n] = l; }
+
+        f32x4 acc[NJ];
 #pragma unroll
-    for (int i = 0; i < NI; i++)
+        for (int j = 0; j < NJ; j++) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+        const uint32_t mine = to - from > (uint32_t)wave ? (to - from - wave + WV - 1) / WV : 0;      // steps of this wave: from + wave, + WV, ..
+        uint32_t ids = NO_PAGE, entries = 0;          // lane e: page and table entry of tile e of the steps looked up last
+        auto look_up = [&](uint32_t k) {              // of steps k .. k + IDS - 1 of this wave
+            const uint32_t step = k + lane / TILES;
+            ids = NO_PAGE;
+            if (step < mine) {
+                const uint64_t tile = (uint64_t)(sp.first + from + wave + step * WV) * TILES + lane % TILES;
+                const uint32_t slot = (uint32_t)(tile >> (kv.shift - 4));
+                entries = slot;
+                if (SEL) entries = slot < a.n_select && slot < pages ? list[slot] : NO_PAGE;
+                if (entries < pages) ids = table[entries];
+                if (ids >= kv.n_pages) ids = NO_PAGE;
+            }
+        };
+        struct Tile {
+            uint32_t pos;          // of its first key, a multiple of 16 (NO_PAGE: no key of it counts)
+            size_t row;            // in the pool
+        };
+        Tile cur[TILES], nxt[TILES];
+        auto find = [&](uint32_t k, Tile (&t)[TILES]) {
 #pragma unroll
-        for (int r = 0; r < 4; r++) sm_o[wave][n][64 * (i / 4) + 4 * (4 * kg + r) + i % 4] = acc[i][r];
-    __syncthreads();
-    for (int e = threadIdx.x; e < g * HD; e += 64 * ATT_W) {
-        const int h = e / HD, d = e % HD;
-        float top = -INFINITY, sum = 0.f, o = 0.f;
-        for (int w = 0; w < ATT_W; w++) top = fmaxf(top, sm_m[w][h]);
-        const float base = top == -INFINITY ? 0.f : top;
-        for (int w = 0; w < ATT_W; w++) {
-            const float f = expf(sm_m[w][h] - base);
-            sum = fmaf(sm_l[w][h], f, sum);
-            o = fmaf(sm_o[w][h][d], f, o);
+            for (int i = 0; i < TILES; i++) {
+                const uint32_t tile = (sp.first + from + wave + k * WV) * TILES + i, e = (k % IDS) * TILES + i;
+                const uint32_t page = __builtin_amdgcn_readlane(ids, e), entry = __builtin_amdgcn_readlane(entries, e);
+                const uint32_t start = (tile & ((1u << (kv.shift - 4)) - 1)) << 4;
+                t[i].pos = page == NO_PAGE ? NO_PAGE : (entry << kv.shift) + start;
+                t[i].row = ((size_t)(page == NO_PAGE ? 0 : page) << kv.shift) + start;
+            }
+        };
+        // rows of a tile: K by lane (key n, dims by kg), V by lane (keys 4 kg + r, dims by n)
+        constexpr int KW = TYPE == FHIP_F32 ? NJ : TYPE == FHIP_Q8_0 ? (NB + 1) / 2 : NB;      // 16-byte words of a lane's part of a key
+        constexpr int VB = HD / 16 * Elem<TYPE>::BYTES;                                       // bytes of a lane's part of a value: 4 .. 32
+        constexpr int VW = VB < 4 ? 1 : VB / 4;
+        uint32_t kr[TILES][KW * 4], vr[TILES][4][VW];
+        uint16_t kd[TYPE == FHIP_Q8_0 ? TILES : 1][4][NB], vd[TYPE == FHIP_Q8_0 ? TILES : 1][4];
+        const size_t row_values = (size_t)kv.n_kv * HD;
+        const uint32_t k_off = (uint32_t)(n * row_values * Elem<TYPE>::BYTES) + (TYPE == FHIP_Q8_0 ? 8 : 16) * kg;
+        auto load_k = [&](const Tile (&t)[TILES]) {
+#pragma unroll
+            for (int i = 0; i < TILES; i++) {
+                const char* base = (const char*)kv.k + (t[i].row * row_values + (size_t)head * HD) * Elem<TYPE>::BYTES;
+                if constexpr (TYPE == FHIP_Q8_0) {
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        const uint2 w = *(const uint2*)(base + k_off + 32 * b);
+                        kr[i][2 * b] = w.x;
+                        kr[i][2 * b + 1] = w.y;
+                    }
+                    const uint16_t* sc = kv.k_scales + (t[i].row * kv.n_kv + head) * NB;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint16_t* s = sc + (uint32_t)(4 * kg + r) * (uint32_t)(kv.n_kv * NB);
+                        if constexpr (NB == 4) {
+                            const uint2 w = *(const uint2*)s;
+                            kd[i][r][0] = (uint16_t)w.x; kd[i][r][1] = (uint16_t)(w.x >> 16);
+                            kd[i][r][2] = (uint16_t)w.y; kd[i][r][3] = (uint16_t)(w.y >> 16);
+                        } else {
+                            const uint32_t w = *(const uint32_t*)s;
+                            kd[i][r][0] = (uint16_t)w; kd[i][r][1] = (uint16_t)(w >> 16);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int b = 0; b < KW; b++) {
+                        const uint4 w = *(const uint4*)(base + k_off + 64 * b);
+                        kr[i][4 * b] = w.x; kr[i][4 * b + 1] = w.y; kr[i][4 * b + 2] = w.z; kr[i][4 * b + 3] = w.w;
+                    }
+                }
+            }
+        };
+        auto load_v = [&](const Tile (&t)[TILES]) {
+#pragma unroll
+            for (int i = 0; i < TILES; i++) {
+                const char* base = (const char*)kv.v + (t[i].row * row_values + (size_t)head * HD) * Elem<TYPE>::BYTES;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const uint32_t off = (uint32_t)((4 * kg + r) * row_values * Elem<TYPE>::BYTES);
+                    if constexpr (TYPE == FHIP_F32) {
+#pragma unroll
+                        for (int h = 0; h < HD / 64; h++) {
+                            const uint4 w = *(const uint4*)(base + off + 256 * h + 16 * n);
+                            vr[i][r][4 * h] = w.x; vr[i][r][4 * h + 1] = w.y; vr[i][r][4 * h + 2] = w.z; vr[i][r][4 * h + 3] = w.w;
+                        }
+                    } else if constexpr (VB == 16) {
+                        const uint4 w = *(const uint4*)(base + off + 16 * n);
+                        vr[i][r][0] = w.x; vr[i][r][1] = w.y; vr[i][r][2] = w.z; vr[i][r][3] = w.w;
+                    } else if constexpr (VB == 8) {
+                        const uint2 w = *(const uint2*)(base + off + 8 * n);
+                        vr[i][r][0] = w.x; vr[i][r][1] = w.y;
+                    } else {
+                        vr[i][r][0] = *(const uint32_t*)(base + off + 4 * n);
+                    }
+                    if constexpr (TYPE == FHIP_Q8_0) vd[i][r] = kv.v_scales[(t[i].row * kv.n_kv + head) * NB + (uint32_t)(4 * kg + r) * (uint32_t)(kv.n_kv * NB) + n / (16 / NB)];
+                }
+            }
+        };
+
+        if (mine > 0) {
+            look_up(0);
+            find(0, cur);
+            load_k(cur);
+            load_v(cur);
         }
-        out[((size_t)seq * n_head + head * g + h) * HD + d] = top == -INFINITY && sum == 0.f ? 0.f : o / sum;      // nothing to attend to: zeros
+        for (uint32_t k = 0; k < mine; k++) {
+            // scores of the step's keys
+            f32x4 s[TILES];
+#pragma unroll
+            for (int i = 0; i < TILES; i++) {
+                s[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                if constexpr (TYPE == FHIP_F32) {
+#pragma unroll
+                    for (int j = 0; j < NJ; j++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[i][4 * j + e]), qf[j][e], s[i], 0, 0, 0);
+                } else if constexpr (TYPE == FHIP_Q8_0) {
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        Frag f;                       // eight codes as f16: 1024 + (c + 128) in the bits, less 1152
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const uint32_t w = kr[i][2 * b + e] ^ 0x80808080u;
+                            const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
+                            f.w[2 * e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - off);
+                            f.w[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - off);
+                        }
+                        f32x4 t = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int p = PARTS - 1; p >= 0; p--) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, qp[b][p].h, t, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) s[i][r] = fmaf(t[r], fhip::kvq_scale(kd[i][r][b]), s[i][r]);
+                    }
+                } else {
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; p--)
+#pragma unroll
+                        for (int b = 0; b < NB; b++) {
+                            Frag f;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) f.w[e] = kr[i][4 * b + e];
+                            if constexpr (TYPE == FHIP_BF16) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.b, qp[b][p].b, s[i], 0, 0, 0);
+                            else s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, qp[b][p].h, s[i], 0, 0, 0);
+                        }
+                }
+            }
+            if (k + 1 < mine) {
+                if ((k + 1) % IDS == 0) look_up(k + 1);
+                find(k + 1, nxt);
+                load_k(nxt);
+            }
+            // softmax: in units of log2; keys that do not count have no weight, and their values, which may be no numbers, are zero
+            if (a.softcap > 0.f) {
+#pragma unroll
+                for (int i = 0; i < TILES; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[i][r] = a.softcap * LOG2E * tanhf(s[i][r] * c2 / a.softcap);
+            } else {
+#pragma unroll
+                for (int i = 0; i < TILES; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[i][r] *= c2;
+            }
+#pragma unroll
+            for (int i = 0; i < TILES; i++)
+                if (cur[i].pos == NO_PAGE || cur[i].pos + 16 > sp.len || cur[i].pos < sp.lo) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const uint32_t key = cur[i].pos + 4 * kg + r;
+                        if (cur[i].pos == NO_PAGE || key >= sp.len || key < sp.lo) {
+                            s[i][r] = -INFINITY;
+#pragma unroll
+                            for (int e = 0; e < VW; e++) vr[i][r][e] = 0;
+                            if (TYPE == FHIP_Q8_0) vd[TYPE == FHIP_Q8_0 ? i : 0][r] = 0;
+                        }
+                    }
+                }
+            float top = s[0][0];
+#pragma unroll
+            for (int i = 0; i < TILES; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) top = fmaxf(top, s[i][r]);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            if (__any(top > m)) {                     // a new maximum in some column
+                const float now = fmaxf(top, m), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - now);
+                m = now;
+                l *= f;
+#pragma unroll
+                for (int j = 0; j < NJ; j++) acc[j] *= f;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+            float p[TILES][4];
+#pragma unroll
+            for (int i = 0; i < TILES; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    p[i][r] = __builtin_amdgcn_exp2f(s[i][r] - base);
+                    l += p[i][r];
+                }
+            // weighted rows
+            if constexpr (P::HALF_V) {
+                Frag pp[PARTS];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    constexpr float UP = TYPE == FHIP_F16 ? 32768.f : 1.f;
+                    uint32_t w[3];
+                    cut<TYPE == FHIP_BF16>(p[x / 2][2 * (x & 1)] * UP, p[x / 2][2 * (x & 1) + 1] * UP, w);
+#pragma unroll
+                    for (int e = 0; e < PARTS; e++) pp[e].w[x] = w[e];
+                }
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    Frag f;
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const uint32_t u = vr[x / 2][2 * (x & 1)][j / 2], w = vr[x / 2][2 * (x & 1) + 1][j / 2];
+                        f.w[x] = j & 1 ? upper_halves(u, w) : lower_halves(u, w);
+                    }
+#pragma unroll
+                    for (int e = PARTS - 1; e >= 0; e--) {
+                        if constexpr (TYPE == FHIP_BF16) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.b, pp[e].b, acc[j], 0, 0, 0);
+                        else acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, pp[e].h, acc[j], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < TILES; i++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float d = TYPE == FHIP_Q8_0 ? fhip::kvq_scale(vd[TYPE == FHIP_Q8_0 ? i : 0][r]) : 1.f;
+#pragma unroll
+                        for (int j = 0; j < NJ; j++) {
+                            const float v = TYPE == FHIP_F32 ? __uint_as_float(vr[i][r][j]) : (float)(int8_t)(vr[i][r][j / 4] >> (8 * (j % 4))) * d;
+                            acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[i][r], acc[j], 0, 0, 0);
+                        }
+                    }
+            }
+            if (k + 1 < mine) {
+                load_v(nxt);
+#pragma unroll
+                for (int i = 0; i < TILES; i++) cur[i] = nxt[i];
+            }
+        }
+        if constexpr (TYPE == FHIP_F16) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++) acc[j] *= 1.f / 32768.f;
+        }
+
+        // the waves' shares joined; element r of acc[j] is dim dim_of(j, 4 kg + r) of head n
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (kg == 0) { sm_m[wave][n] = m; sm_l[wave][n] = l; }
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int j = 0; j < NJ; j += 4) {
+                const int d = TYPE == FHIP_F32 ? 16 * j + 4 * (4 * kg + r) : NJ * (4 * kg + r) + j;
+                *(f32x4*)&sm_o[wave][n][d] = (f32x4){acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
+            }
+        __syncthreads();
+        const bool whole = from == 0 && to == sp.steps;
+        float* part = whole ? nullptr : a.part + ((size_t)blockIdx.x * 2 + (at == range0 ? 0 : 1)) * g * (HD + 4);
+        for (int e = threadIdx.x; e < g * (HD / 4); e += 64 * WV) {
+            const int h = e / (HD / 4), d = 4 * (e % (HD / 4));
+            float top = sm_m[0][h], sum = 0.f;
+#pragma unroll
+            for (int w = 1; w < WV; w++) top = fmaxf(top, sm_m[w][h]);
+            const float base = top == -INFINITY ? 0.f : top;
+            f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < WV; w++) {
+                const float f = __builtin_amdgcn_exp2f(sm_m[w][h] - base);
+                sum = fmaf(sm_l[w][h], f, sum);
+                o += *(const f32x4*)&sm_o[w][h][d] * f;
+            }
+            if (whole) {
+                const float inv = top == -INFINITY && sum == 0.f ? 0.f : 1.f / sum;      // nothing to attend to: zeros
+                *(f32x4*)(a.out + ((size_t)seq * a.n_head + head * g + h) * HD + d) = o * inv;
+            } else {
+                *(f32x4*)(part + h * HD + d) = o;
+                if (d == 0) { part[g * HD + 2 * h] = top; part[g * HD + 2 * h + 1] = sum; }
+            }
+        }
+        if (a.log_wgs < 0) return;
+        at += to - from;
+        if (at >= end) return;
+        // the next unit: the sequence's next KV head, or the next sequence with any steps
+        from = 0;
+        if (++head == (uint32_t)kv.n_kv) {
+            head = 0;
+            do {
+                if (seq + 1 >= kv.n_seq) return;
+                sp = span_of<TYPE, SEL>(kv, a.lens, ++seq, a.max_len, a.window, a.n_select);
+            } while (sp.steps == 0);
+        }
+        __syncthreads();
+    }
+}
+
+// What the workgroups of a unit that was cut have left, added in their order; zeros for a unit without keys. A workgroup a query head.
+template <int TYPE, int HD, bool SEL>
+__global__ __launch_bounds__(256) void join_kernel(Attend a) {
+    constexpr int LANES = HD / 4, GROUPS = 256 / LANES;
+    __shared__ float sm_top[4], sm_l[GROUPS];
+    __shared__ __attribute__((aligned(16))) float sm_o[GROUPS][HD];
+    const PagedView& kv = a.kv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = a.n_head / kv.n_kv;
+    const uint32_t seq = blockIdx.x / a.n_head, qh = blockIdx.x % a.n_head, head = qh / g, h = qh % g;
+    uint64_t all = 0, before = 0;
+    for (uint32_t b = 0; b < kv.n_seq; b += 64) {
+        const uint64_t c = b + lane < kv.n_seq ? (uint64_t)span_of<TYPE, SEL>(kv, a.lens, b + lane, a.max_len, a.window, a.n_select).steps * kv.n_kv : 0;
+        const uint64_t upto = wave_scan(c, lane);
+        if (seq >= b && seq < b + 64) before = all + __shfl((unsigned long long)(upto - c), seq - b);
+        all += __shfl((unsigned long long)upto, 63);
+    }
+    const uint64_t per = steps_each(all, a.log_wgs, a.min_steps);
+    const Span sp = span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select);
+    float* out = a.out + ((size_t)seq * a.n_head + qh) * HD;
+    if (sp.steps == 0) {
+        if (threadIdx.x < HD) out[threadIdx.x] = 0.f;
+        return;
+    }
+    const uint64_t u0 = before + (uint64_t)head * sp.steps, u1 = u0 + sp.steps;
+    const uint32_t w0 = (uint32_t)(u0 / per), w1 = (uint32_t)((u1 - 1) / per);
+    if (w0 == w1) return;                             // the unit lies within one range: finished there
+    auto part = [&](uint32_t w) { return a.part + ((size_t)w * 2 + (w == w0 && u0 > w * per ? 1 : 0)) * g * (HD + 4); };
+    float top = -INFINITY;
+    for (uint32_t w = w0 + threadIdx.x; w <= w1; w += 256) top = fmaxf(top, part(w)[g * HD + 2 * h]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if (lane == 0) sm_top[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(sm_top[0], sm_top[1]), fmaxf(sm_top[2], sm_top[3]));
+    const float base = top == -INFINITY ? 0.f : top;
+    const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
+    f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f;
+    for (uint32_t w = w0 + group; w <= w1; w += GROUPS) {
+        const float* p = part(w);
+        const float f = __builtin_amdgcn_exp2f(p[g * HD + 2 * h] - base);
+        sum = fmaf(p[g * HD + 2 * h + 1], f, sum);
+        o += *(const f32x4*)(p + h * HD + d) * f;
+    }
+    *(f32x4*)&sm_o[group][d] = o;
+    if (d == 0) sm_l[group] = sum;
+    __syncthreads();
+    if (threadIdx.x < HD) {
+        float v = 0.f, t = 0.f;
+#pragma unroll
+        for (int i = 0; i < GROUPS; i++) {
+            v += sm_o[i][threadIdx.x];
+            t += sm_l[i];
+        }
+        out[threadIdx.x] = top == -INFINITY && t == 0.f ? 0.f : v / t;
     }
 }
 
@@ -550,17 +1015,28 @@ int launch_paged_select(int hd, const PagedView& kv, const float* q, const uint3
     return check_hip(hipGetLastError(), "paged_select launch");
 }
 
-size_t paged_attention_ws_bytes(const PagedView&, int, int, size_t) { return 0; }
+// Workgroups that the steps are dealt out to, two a CU; a launch whose units hold no more than UNCUT keys has a workgroup for each and nothing to join.
+constexpr int LOG_WGS = 9, UNCUT = 512, MIN_STEPS = 8;
+size_t paged_attention_ws_bytes(const PagedView& kv, int hd, int n_head, size_t max_len) {
+    return max_len <= UNCUT ? 0 : ((size_t)2 << LOG_WGS) * (n_head / kv.n_kv) * (hd + 4) * sizeof(float);
+}
 int launch_paged_attention(uint32_t type, int hd, const PagedView& kv, const float* q, const uint32_t* lens, uint32_t max_len, const uint32_t* selected, uint32_t n_select,
                            int n_head, uint32_t window, float softcap, float* ws, float* out, hipStream_t s) {
-    (void)ws;
-    const float scale = 1.0f / sqrtf((float)hd);
-    const dim3 grid(kv.n_seq * kv.n_kv);
+    Attend a;
+    a.kv = kv; a.q = q; a.lens = lens; a.selected = selected; a.out = out; a.part = ws;
+    a.max_len = max_len; a.n_select = n_select; a.window = window; a.n_head = n_head; a.softcap = softcap; a.scale = 1.0f / sqrtf((float)hd);
+    const size_t keys = selected ? (size_t)n_select << kv.shift : max_len;
+    a.log_wgs = keys <= UNCUT ? -1 : LOG_WGS;
+    a.min_steps = MIN_STEPS;
+    const dim3 grid(a.log_wgs < 0 ? kv.n_seq * kv.n_kv : 1u << LOG_WGS);
     return by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
-        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(64 * ATT_W), 0, s, kv, q, lens, max_len, selected, n_select, n_head, window, softcap, scale, out); };
-        if (hd == 128) selected ? go(attention_kernel<TYPE, 128, true>) : go(attention_kernel<TYPE, 128, false>);
-        else selected ? go(attention_kernel<TYPE, 64, true>) : go(attention_kernel<TYPE, 64, false>);
+        auto go = [&](auto kernel, auto join) {
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a);
+            if (a.log_wgs >= 0) hipLaunchKernelGGL(join, dim3(kv.n_seq * (unsigned)n_head), dim3(256), 0, s, a);
+        };
+        if (hd == 128) selected ? go(attention_kernel<TYPE, 128, true, 4>, join_kernel<TYPE, 128, true>) : go(attention_kernel<TYPE, 128, false, 4>, join_kernel<TYPE, 128, false>);
+        else selected ? go(attention_kernel<TYPE, 64, true, 4>, join_kernel<TYPE, 64, true>) : go(attention_kernel<TYPE, 64, false, 4>, join_kernel<TYPE, 64, false>);
         return check_hip(hipGetLastError(), "paged_attention launch");
     });
 }

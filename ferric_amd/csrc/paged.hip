@@ -428,6 +428,32 @@ __device__ __forceinline__ void cut(float a, float b, uint32_t (&w)[3]) {
     }
 }
 
+// tanh of four scores over their cap, which is small for nearly all of them: its series up to y^17 within 1/2 (what is left out is 3e-10 of it there), otherwise 1 - 2 / (1 + e^2y), whose
+// cancellation costs a factor of two there at most. The library's tanhf, two branches a value that a wave takes both, was half of a capped launch: 33 sequences, window 1024,
+// 16 heads of 64 on Q8_0 81.7 us a pass with it.
+__device__ __forceinline__ f32x4 tanh4(f32x4 y) {
+    const f32x4 z = y * y;
+    f32x4 t = z * (6404582.f / 10854718875.f) - 929569.f / 638512875.f;
+    t = t * z + 21844.f / 6081075.f;
+    t = t * z - 1382.f / 155925.f;
+    t = t * z + 62.f / 2835.f;
+    t = t * z - 17.f / 315.f;
+    t = t * z + 2.f / 15.f;
+    t = t * z - 1.f / 3.f;
+    t = y * z * t + y;
+    float far = 0.f;
+#pragma unroll
+    for (int r = 0; r < 4; r++) far = fmaxf(far, fabsf(y[r]));
+    if (__any(!(far < 0.5f))) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const float big = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(fabsf(y[r]) * (2.f * LOG2E)));
+            t[r] = fabsf(y[r]) < 0.5f ? t[r] : copysignf(big, y[r]);
+        }
+    }
+    return t;
+}
+
 template <int TYPE>
 struct Path {
     static constexpr int TILES = TYPE == FHIP_F32 ? 1 : 2;            // of 16 keys a step
@@ -457,6 +483,10 @@ __device__ __forceinline__ Span span_of(const PagedView& kv, const uint32_t* __r
     }
     return s;
 }
+// The same in scalar registers, where it is the same for the whole wave.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t uniform(uint64_t v) { return (uint64_t)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v); }
+__device__ __forceinline__ Span uniform(Span s) { return Span{uniform(s.len), uniform(s.lo), uniform(s.first), uniform(s.steps)}; }
 // Steps in front of sequence 64 b + lane in blocks of 64 sequences, and of all: a wave's scan.
 __device__ __forceinline__ uint64_t wave_scan(uint64_t v, int lane) {      // inclusive
 #pragma unroll
@@ -513,9 +543,9 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
     if (a.log_wgs < 0) {
         seq = blockIdx.x / kv.n_kv;
         head = blockIdx.x % kv.n_kv;
-        sp = span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select);
+        sp = uniform(span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select));
     } else {
-        const uint64_t all = all_steps<TYPE, SEL>(a, lane), per = steps_each(all, a.log_wgs, a.min_steps);
+        const uint64_t all = uniform(all_steps<TYPE, SEL>(a, lane)), per = steps_each(all, a.log_wgs, a.min_steps);
         at = blockIdx.x * per;
         end = at + per < all ? at + per : all;
         if (at >= end) return;
@@ -531,65 +561,21 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
             }
             before = __shfl((unsigned long long)upto, 63);
         }
-        seq = __builtin_amdgcn_readfirstlane(seq);
-        sp = span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select);
-        head = (uint32_t)((at - unit0) / sp.steps);
-        from = (uint32_t)((at - unit0) - (uint64_t)head * sp.steps);
+        seq = uniform(seq);
+        unit0 = uniform(unit0);
+        sp = uniform(span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select));
+        head = uniform((uint32_t)((at - unit0) / sp.steps));
+        from = uniform((uint32_t)((at - unit0) - (uint64_t)head * sp.steps));
     }
     const uint64_t range0 = at;
 
     for (;;) {
-        head = __builtin_amdgcn_readfirstlane(head);
         const uint32_t to = a.log_wgs < 0 || end - at > sp.steps - from ? sp.steps : from + (uint32_t)(end - at);   // steps [from, to) of the unit
         const uint32_t* table = kv.table + seq * kv.table_stride;
         const uint32_t* list = SEL ? a.selected + ((size_t)seq * kv.n_kv + head) * a.n_select : nullptr;
         const uint32_t pages = pages_of(kv, sp.len);
 
-        // the unit's queries, as the second operand of K q^T
-        float m = -INFINITY, l = 0.f, c2 = a.scale * (a.softcap > 0.f ? 1.f : LOG2E);
-        f32x4 qf[P::HALF ? 1 : NJ];
-        Frag qp[P::HALF ? NB : 1][P::HALF ? PARTS : 1];
-        {
-            const float* qh = a.q + ((size_t)seq * a.n_head + head * g + (n < g ? n : 0)) * HD;
-            if constexpr (!P::HALF) {
-#pragma unroll
-                for (int i = 0; i < NJ; i++) {
-                    qf[i] = *(const f32x4*)(qh + 16 * i + 4 * kg);
-                    if (n >= g) qf[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-                }
-            } else {
-                f32x4 raw[NB][2];
-                float top = 0.f;
-#pragma unroll
-                for (int i = 0; i < NB; i++)
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        raw[i][e] = *(const f32x4*)(qh + 32 * i + 8 * kg + 4 * e);
-                        if (n >= g) raw[i][e] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int x = 0; x < 4; x++) top = fmaxf(top, fabsf(raw[i][e][x]));
-                    }
-                float up = 1.f;
-                if constexpr (TYPE != FHIP_BF16) {     // the head's largest |q| to [2^14, 2^15)
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    const int ex = top > 0.f && top < INFINITY ? 14 - (int)(((__float_as_uint(top) >> 23) & 255u) - 127u) : 0;
-                    const int clipped = ex < -126 ? -126 : ex > 126 ? 126 : ex;
-                    up = __uint_as_float((uint32_t)(127 + clipped) << 23);
-                    c2 *= __uint_as_float((uint32_t)(127 - clipped) << 23);
-                }
-#pragma unroll
-                for (int i = 0; i < NB; i++)
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        uint32_t w[3];
-                        cut<TYPE == FHIP_BF16>(raw[i][x / 2][2 * (x & 1)] * up, raw[i][x / 2][2 * (x & 1) + 1] * up, w);
-#pragma unroll
-                        for (int p = 0; p < PARTS; p++) qp[i][p].w[x] = w[p];
-                    }
-            }
-        }
-
+        float m = -INFINITY, l = 0.f, c2 = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E;
         f32x4 acc[NJ];
 #pragma unroll
         for (int j = 0; j < NJ; j++) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -691,13 +677,50 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
             }
         };
 
-        if (mine > 0) {
-            look_up(0);
-            find(0, cur);
-            load_k(cur);
-            load_v(cur);
-        }
-        for (uint32_t k = 0; k < mine; k++) {
+        // the unit's queries, as the second operand of K q^T
+        f32x4 raw[NJ];
+        f32x4 qf[P::HALF ? 1 : NJ];
+        Frag qp[P::HALF ? NB : 1][P::HALF ? PARTS : 1];
+        auto load_q = [&] {
+            const float* qh = a.q + ((size_t)seq * a.n_head + head * g + (n < g ? n : 0)) * HD;
+#pragma unroll
+            for (int i = 0; i < NJ; i++) raw[i] = *(const f32x4*)(qh + (P::HALF ? 32 * (i / 2) + 8 * kg + 4 * (i & 1) : 16 * i + 4 * kg));
+        };
+        auto take_q = [&] {
+#pragma unroll
+            for (int i = 0; i < NJ; i++)
+                if (n >= g) raw[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if constexpr (!P::HALF) {
+#pragma unroll
+                for (int i = 0; i < NJ; i++) qf[i] = raw[i];
+            } else {
+                float up = 1.f;
+                if constexpr (TYPE != FHIP_BF16) {     // the head's largest |q| to [2^14, 2^15)
+                    float top = 0.f;
+#pragma unroll
+                    for (int i = 0; i < NJ; i++)
+#pragma unroll
+                        for (int x = 0; x < 4; x++) top = fmaxf(top, fabsf(raw[i][x]));
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const int ex = top > 0.f && top < INFINITY ? 14 - (int)(((__float_as_uint(top) >> 23) & 255u) - 127u) : 0;
+                    const int clipped = ex < -126 ? -126 : ex > 126 ? 126 : ex;
+                    up = __uint_as_float((uint32_t)(127 + clipped) << 23);
+                    c2 *= __uint_as_float((uint32_t)(127 - clipped) << 23);
+                }
+#pragma unroll
+                for (int i = 0; i < NB; i++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        uint32_t w[3];
+                        cut<TYPE == FHIP_BF16>(raw[2 * i + x / 2][2 * (x & 1)] * up, raw[2 * i + x / 2][2 * (x & 1) + 1] * up, w);
+#pragma unroll
+                        for (int p = 0; p < PARTS; p++) qp[i][p].w[x] = w[p];
+                    }
+            }
+        };
+        // A step, and what it requests of the next one: as two copies, since a request under a condition would be waited for wherever the other path could come from.
+        auto work = [&](uint32_t k, auto more) {
             // scores of the step's keys
             f32x4 s[TILES];
 #pragma unroll
@@ -738,7 +761,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                         }
                 }
             }
-            if (k + 1 < mine) {
+            if constexpr (more()) {
                 if ((k + 1) % IDS == 0) look_up(k + 1);
                 find(k + 1, nxt);
                 load_k(nxt);
@@ -746,9 +769,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
             // softmax: in units of log2; keys that do not count have no weight, and their values, which may be no numbers, are zero
             if (a.softcap > 0.f) {
 #pragma unroll
-                for (int i = 0; i < TILES; i++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) s[i][r] = a.softcap * LOG2E * tanhf(s[i][r] * c2 / a.softcap);
+                for (int i = 0; i < TILES; i++) s[i] = tanh4(s[i] * c2) * (a.softcap * LOG2E);
             } else {
 #pragma unroll
                 for (int i = 0; i < TILES; i++)
@@ -830,11 +851,23 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                         }
                     }
             }
-            if (k + 1 < mine) {
+            if constexpr (more()) {
                 load_v(nxt);
 #pragma unroll
                 for (int i = 0; i < TILES; i++) cur[i] = nxt[i];
             }
+        };
+        if (mine > 0) {
+            load_q();
+            look_up(0);
+            find(0, cur);
+            load_k(cur);
+            __builtin_amdgcn_sched_barrier(0);        // in the loop's order: the wait for the first keys is not one for the values
+            load_v(cur);
+            __builtin_amdgcn_sched_barrier(0);
+            take_q();
+            for (uint32_t k = 0; k + 1 < mine; k++) work(k, std::true_type());
+            work(mine - 1, std::false_type());
         }
         if constexpr (TYPE == FHIP_F16) {
 #pragma unroll
@@ -885,7 +918,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
             head = 0;
             do {
                 if (seq + 1 >= kv.n_seq) return;
-                sp = span_of<TYPE, SEL>(kv, a.lens, ++seq, a.max_len, a.window, a.n_select);
+                sp = uniform(span_of<TYPE, SEL>(kv, a.lens, ++seq, a.max_len, a.window, a.n_select));
             } while (sp.steps == 0);
         }
         __syncthreads();

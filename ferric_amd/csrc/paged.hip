@@ -392,7 +392,9 @@ __global__ __launch_bounds__(SEL_T) void select_kernel(PagedView kv, const uint3
 //   f32    v_mfma_f32_16x16x4_f32 on the rows as they are.
 //   bf16   v_mfma_f32_16x16x32_bf16; q and p as three bf16 values each, cut off rather than rounded, so that they add up to the f32 value.
 //   f16    v_mfma_f32_16x16x32_f16; q (times a power of two that brings its largest value to 2^14) and p (times 2^15) as two f16 values, 22 bits.
-//   Q8_0   keys as f16 holds their codes, q as for f16, a block of 32 dims an instruction, whose sum is multiplied by the block's scale; values as c * d on the f32 instruction.
+//   Q8_0   keys as f16 holds their codes, q as for f16, a block of 32 dims an instruction, whose sum is multiplied by the block's scale; values c * d, 8 by 11 bits, as the two f16 values
+//          whose sum they are, p times 2^7 as two (three products: the two small parts' is 2^-22 of the result). On the f32 instruction, which takes four keys where
+//          these take 32, a capped window of 33 sequences, 16 heads of 64, took 69 us.
 // Bound by the rows' bytes. The next step's keys are requested once the current ones are multiplied, its values once the current ones are: eight waves a CU keep 64 KB and more
 // on the way without a second set of registers.
 //
@@ -411,6 +413,18 @@ union Frag {
 // the upper halves of two words, the first one's in the lower half
 __device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 __device__ __forceinline__ uint32_t lower_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+// the largest of a column's four lanes, in all of them
+__device__ __forceinline__ float column_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// Two codes of a Q8_0 block as f16: byte c + 128 in the bits of 1024 + c + 128, less 1152. sel: 0x04ii04jj for bytes j and i.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t sel) {
+    const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, sel)) - off);
+}
 // Two f32 as PARTS 16-bit values each: word i of the result holds part i of both.
 template <bool BF>
 __device__ __forceinline__ void cut(float a, float b, uint32_t (&w)[3]) {
@@ -459,8 +473,7 @@ struct Path {
     static constexpr int TILES = TYPE == FHIP_F32 ? 1 : 2;            // of 16 keys a step
     static constexpr int KEYS = 16 * TILES;
     static constexpr int PARTS = TYPE == FHIP_BF16 ? 3 : 2;
-    static constexpr bool HALF = TYPE != FHIP_F32;                    // K on a 16-bit instruction
-    static constexpr bool HALF_V = TYPE == FHIP_BF16 || TYPE == FHIP_F16;
+    static constexpr bool HALF = TYPE != FHIP_F32;                    // on a 16-bit instruction
 };
 
 // Keys of sequence `seq` that are attended to, [lo, len), and the steps that they lie in.
@@ -573,7 +586,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
         const uint32_t to = a.log_wgs < 0 || end - at > sp.steps - from ? sp.steps : from + (uint32_t)(end - at);   // steps [from, to) of the unit
         const uint32_t* table = kv.table + seq * kv.table_stride;
         const uint32_t* list = SEL ? a.selected + ((size_t)seq * kv.n_kv + head) * a.n_select : nullptr;
-        const uint32_t pages = pages_of(kv, sp.len);
+        const uint32_t pages = pages_of(kv, sp.len), row_values = (uint32_t)kv.n_kv * HD;
 
         float m = -INFINITY, l = 0.f, c2 = a.softcap > 0.f ? a.scale / a.softcap : a.scale * LOG2E;
         f32x4 acc[NJ];
@@ -581,32 +594,34 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
         for (int j = 0; j < NJ; j++) acc[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
         const uint32_t mine = to - from > (uint32_t)wave ? (to - from - wave + WV - 1) / WV : 0;      // steps of this wave: from + wave, + WV, ..
-        uint32_t ids = NO_PAGE, entries = 0;          // lane e: page and table entry of tile e of the steps looked up last
+        // Lane e: tile e of the steps looked up last, its first key's position and its row's first value in the pools.
+        uint32_t tile_pos = NO_PAGE;
+        uint64_t tile_at = 0;
         auto look_up = [&](uint32_t k) {              // of steps k .. k + IDS - 1 of this wave
             const uint32_t step = k + lane / TILES;
-            ids = NO_PAGE;
+            uint32_t page = NO_PAGE, entry = 0, start = 0;
             if (step < mine) {
-                const uint64_t tile = (uint64_t)(sp.first + from + wave + step * WV) * TILES + lane % TILES;
-                const uint32_t slot = (uint32_t)(tile >> (kv.shift - 4));
-                entries = slot;
-                if (SEL) entries = slot < a.n_select && slot < pages ? list[slot] : NO_PAGE;
-                if (entries < pages) ids = table[entries];
-                if (ids >= kv.n_pages) ids = NO_PAGE;
+                const uint32_t tile = (sp.first + from + wave + step * WV) * TILES + lane % TILES, slot = tile >> (kv.shift - 4);
+                start = (tile & ((1u << (kv.shift - 4)) - 1)) << 4;
+                entry = slot;
+                if (SEL) entry = slot < a.n_select && slot < pages ? list[slot] : NO_PAGE;
+                if (entry < pages) page = table[entry];
             }
+            const bool none = page >= kv.n_pages;     // its place in page 0 is read and counts for nothing
+            tile_pos = none ? NO_PAGE : (entry << kv.shift) + start;
+            tile_at = (((uint64_t)(none ? 0 : page) << kv.shift) + start) * row_values + (uint32_t)head * HD;
         };
         struct Tile {
             uint32_t pos;          // of its first key, a multiple of 16 (NO_PAGE: no key of it counts)
-            size_t row;            // in the pool
+            uint64_t at;           // the KV head's first value of that key
         };
         Tile cur[TILES], nxt[TILES];
         auto find = [&](uint32_t k, Tile (&t)[TILES]) {
 #pragma unroll
             for (int i = 0; i < TILES; i++) {
-                const uint32_t tile = (sp.first + from + wave + k * WV) * TILES + i, e = (k % IDS) * TILES + i;
-                const uint32_t page = __builtin_amdgcn_readlane(ids, e), entry = __builtin_amdgcn_readlane(entries, e);
-                const uint32_t start = (tile & ((1u << (kv.shift - 4)) - 1)) << 4;
-                t[i].pos = page == NO_PAGE ? NO_PAGE : (entry << kv.shift) + start;
-                t[i].row = ((size_t)(page == NO_PAGE ? 0 : page) << kv.shift) + start;
+                const uint32_t e = (k % IDS) * TILES + i;
+                t[i].pos = __builtin_amdgcn_readlane(tile_pos, e);
+                t[i].at = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(tile_at >> 32), e) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)tile_at, e);
             }
         };
         // rows of a tile: K by lane (key n, dims by kg), V by lane (keys 4 kg + r, dims by n)
@@ -614,49 +629,46 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
         constexpr int VB = HD / 16 * Elem<TYPE>::BYTES;                                       // bytes of a lane's part of a value: 4 .. 32
         constexpr int VW = VB < 4 ? 1 : VB / 4;
         uint32_t kr[TILES][KW * 4], vr[TILES][4][VW];
-        uint16_t kd[TYPE == FHIP_Q8_0 ? TILES : 1][4][NB], vd[TYPE == FHIP_Q8_0 ? TILES : 1][4];
-        const size_t row_values = (size_t)kv.n_kv * HD;
+        uint32_t kd[TYPE == FHIP_Q8_0 ? TILES : 1][4][NB / 2];      // two scales a word
+        uint16_t vd[TYPE == FHIP_Q8_0 ? TILES : 1][4];
         const uint32_t k_off = (uint32_t)(n * row_values * Elem<TYPE>::BYTES) + (TYPE == FHIP_Q8_0 ? 8 : 16) * kg;
+        // (the parts of both tiles in turn, as the products take them)
         auto load_k = [&](const Tile (&t)[TILES]) {
+            if constexpr (TYPE == FHIP_Q8_0) {
 #pragma unroll
-            for (int i = 0; i < TILES; i++) {
-                const char* base = (const char*)kv.k + (t[i].row * row_values + (size_t)head * HD) * Elem<TYPE>::BYTES;
-                if constexpr (TYPE == FHIP_Q8_0) {
-#pragma unroll
-                    for (int b = 0; b < NB; b++) {
-                        const uint2 w = *(const uint2*)(base + k_off + 32 * b);
-                        kr[i][2 * b] = w.x;
-                        kr[i][2 * b + 1] = w.y;
-                    }
-                    const uint16_t* sc = kv.k_scales + (t[i].row * kv.n_kv + head) * NB;
+                for (int i = 0; i < TILES; i++)
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const uint16_t* s = sc + (uint32_t)(4 * kg + r) * (uint32_t)(kv.n_kv * NB);
+                        const uint16_t* s = kv.k_scales + (t[i].at >> 5) + (uint32_t)(4 * kg + r) * (row_values / 32);
                         if constexpr (NB == 4) {
                             const uint2 w = *(const uint2*)s;
-                            kd[i][r][0] = (uint16_t)w.x; kd[i][r][1] = (uint16_t)(w.x >> 16);
-                            kd[i][r][2] = (uint16_t)w.y; kd[i][r][3] = (uint16_t)(w.y >> 16);
+                            kd[i][r][0] = w.x; kd[i][r][1] = w.y;
                         } else {
-                            const uint32_t w = *(const uint32_t*)s;
-                            kd[i][r][0] = (uint16_t)w; kd[i][r][1] = (uint16_t)(w >> 16);
+                            kd[i][r][0] = *(const uint32_t*)s;
                         }
                     }
-                } else {
+            }
 #pragma unroll
-                    for (int b = 0; b < KW; b++) {
-                        const uint4 w = *(const uint4*)(base + k_off + 64 * b);
+            for (int b = 0; b < (TYPE == FHIP_Q8_0 ? NB : KW); b++)
+#pragma unroll
+                for (int i = 0; i < TILES; i++) {
+                    const char* base = (const char*)kv.k + t[i].at * Elem<TYPE>::BYTES + k_off;
+                    if constexpr (TYPE == FHIP_Q8_0) {
+                        const uint2 w = *(const uint2*)(base + 32 * b);
+                        kr[i][2 * b] = w.x; kr[i][2 * b + 1] = w.y;
+                    } else {
+                        const uint4 w = *(const uint4*)(base + 64 * b);
                         kr[i][4 * b] = w.x; kr[i][4 * b + 1] = w.y; kr[i][4 * b + 2] = w.z; kr[i][4 * b + 3] = w.w;
                     }
                 }
-            }
         };
         auto load_v = [&](const Tile (&t)[TILES]) {
 #pragma unroll
             for (int i = 0; i < TILES; i++) {
-                const char* base = (const char*)kv.v + (t[i].row * row_values + (size_t)head * HD) * Elem<TYPE>::BYTES;
+                const char* base = (const char*)kv.v + t[i].at * Elem<TYPE>::BYTES;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const uint32_t off = (uint32_t)((4 * kg + r) * row_values * Elem<TYPE>::BYTES);
+                    const uint32_t off = (4 * kg + r) * row_values * Elem<TYPE>::BYTES;
                     if constexpr (TYPE == FHIP_F32) {
 #pragma unroll
                         for (int h = 0; h < HD / 64; h++) {
@@ -672,7 +684,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                     } else {
                         vr[i][r][0] = *(const uint32_t*)(base + off + 4 * n);
                     }
-                    if constexpr (TYPE == FHIP_Q8_0) vd[i][r] = kv.v_scales[(t[i].row * kv.n_kv + head) * NB + (uint32_t)(4 * kg + r) * (uint32_t)(kv.n_kv * NB) + n / (16 / NB)];
+                    if constexpr (TYPE == FHIP_Q8_0) vd[i][r] = kv.v_scales[(t[i].at >> 5) + (uint32_t)(4 * kg + r) * (row_values / 32) + n / (16 / NB)];
                 }
             }
         };
@@ -701,8 +713,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                     for (int i = 0; i < NJ; i++)
 #pragma unroll
                         for (int x = 0; x < 4; x++) top = fmaxf(top, fabsf(raw[i][x]));
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
+                    top = column_max(top);
                     const int ex = top > 0.f && top < INFINITY ? 14 - (int)(((__float_as_uint(top) >> 23) & 255u) - 127u) : 0;
                     const int clipped = ex < -126 ? -126 : ex > 126 ? 126 : ex;
                     up = __uint_as_float((uint32_t)(127 + clipped) << 23);
@@ -724,42 +735,52 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
             // scores of the step's keys
             f32x4 s[TILES];
 #pragma unroll
-            for (int i = 0; i < TILES; i++) {
-                s[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
-                if constexpr (TYPE == FHIP_F32) {
+            for (int i = 0; i < TILES; i++) s[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            if constexpr (TYPE == FHIP_F32) {
+                f32x4 s2 = (f32x4){0.f, 0.f, 0.f, 0.f};      // two chains: half of the products' latency
 #pragma unroll
-                    for (int j = 0; j < NJ; j++)
+                for (int j = 0; j < NJ; j++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) s[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[i][4 * j + e]), qf[j][e], s[i], 0, 0, 0);
-                } else if constexpr (TYPE == FHIP_Q8_0) {
+                    for (int e = 0; e < 4; e++) {
+                        f32x4& t = e & 1 ? s2 : s[0];
+                        t = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[0][4 * j + e]), qf[j][e], t, 0, 0, 0);
+                    }
+                s[0] += s2;
+            } else if constexpr (TYPE == FHIP_Q8_0) {
 #pragma unroll
-                    for (int b = 0; b < NB; b++) {
-                        Frag f;                       // eight codes as f16: 1024 + (c + 128) in the bits, less 1152
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int i = 0; i < TILES; i++) {
+                        Frag f;                       // eight codes
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             const uint32_t w = kr[i][2 * b + e] ^ 0x80808080u;
-                            const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
-                            f.w[2 * e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) - off);
-                            f.w[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) - off);
+                            f.w[2 * e] = codes_f16(w, 0x04010400u);
+                            f.w[2 * e + 1] = codes_f16(w, 0x04030402u);
                         }
                         f32x4 t = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int p = PARTS - 1; p >= 0; p--) t = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, qp[b][p].h, t, 0, 0, 0);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) s[i][r] = fmaf(t[r], fhip::kvq_scale(kd[i][r][b]), s[i][r]);
+                        for (int r = 0; r < 4; r++) {
+                            const f16x2 d = __builtin_bit_cast(f16x2, kd[i][r][b / 2]);
+                            s[i][r] = fmaf(t[r], (float)(b & 1 ? d.y : d.x), s[i][r]);
+                        }
                     }
-                } else {
+            } else {
+                // the small parts of q first: each chunk's products as its keys come in
+#pragma unroll
+                for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int p = PARTS - 1; p >= 0; p--)
 #pragma unroll
-                        for (int b = 0; b < NB; b++) {
+                        for (int i = 0; i < TILES; i++) {
                             Frag f;
 #pragma unroll
                             for (int e = 0; e < 4; e++) f.w[e] = kr[i][4 * b + e];
                             if constexpr (TYPE == FHIP_BF16) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.b, qp[b][p].b, s[i], 0, 0, 0);
                             else s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, qp[b][p].h, s[i], 0, 0, 0);
                         }
-                }
             }
             if constexpr (more()) {
                 if ((k + 1) % IDS == 0) look_up(k + 1);
@@ -795,8 +816,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
             for (int i = 0; i < TILES; i++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) top = fmaxf(top, s[i][r]);
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
+            top = column_max(top);
             if (__any(top > m)) {                     // a new maximum in some column
                 const float now = fmaxf(top, m), f = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - now);
                 m = now;
@@ -814,24 +834,51 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                     l += p[i][r];
                 }
             // weighted rows
-            if constexpr (P::HALF_V) {
+            if constexpr (P::HALF) {
+                float up = TYPE == FHIP_F16 ? 32768.f : TYPE == FHIP_Q8_0 ? 128.f : 1.f;
+                uint32_t d2[TYPE == FHIP_Q8_0 ? 4 : 1];      // Q8_0: the scales of keys 2 x and 2 x + 1 in the lane's order
+                if constexpr (TYPE == FHIP_Q8_0) {
+                    uint32_t big = 0;
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const uint16_t u = vd[x / 2][2 * (x & 1)], w = vd[x / 2][2 * (x & 1) + 1];
+                        d2[x] = (uint32_t)u | (uint32_t)w << 16;
+                        big |= (u > 0x5FFFu) | (w > 0x5FFFu);      // 512 and more (or no number): c * d would leave f16
+                    }
+                    if (__any(big)) {                 // a 256th of the scales, 256 times the weights
+                        up = 32768.f;
+#pragma unroll
+                        for (int x = 0; x < 4; x++) d2[x] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, d2[x]) * (f16x2){(_Float16)(1.f / 256.f), (_Float16)(1.f / 256.f)});
+                    }
+                }
                 Frag pp[PARTS];
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
-                    constexpr float UP = TYPE == FHIP_F16 ? 32768.f : 1.f;
                     uint32_t w[3];
-                    cut<TYPE == FHIP_BF16>(p[x / 2][2 * (x & 1)] * UP, p[x / 2][2 * (x & 1) + 1] * UP, w);
+                    cut<TYPE == FHIP_BF16>(p[x / 2][2 * (x & 1)] * up, p[x / 2][2 * (x & 1) + 1] * up, w);
 #pragma unroll
                     for (int e = 0; e < PARTS; e++) pp[e].w[x] = w[e];
                 }
 #pragma unroll
                 for (int j = 0; j < NJ; j++) {
-                    Frag f;
+                    Frag f, lo;
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
-                        const uint32_t u = vr[x / 2][2 * (x & 1)][j / 2], w = vr[x / 2][2 * (x & 1) + 1][j / 2];
-                        f.w[x] = j & 1 ? upper_halves(u, w) : lower_halves(u, w);
+                        const int i = x / 2, r = 2 * (x & 1);
+                        if constexpr (TYPE == FHIP_Q8_0) {
+                            // values j of two keys: c * d = f + lo, exactly
+                            const uint32_t both = __builtin_amdgcn_perm(vr[i][r + 1][j / 4] ^ 0x80808080u, vr[i][r][j / 4] ^ 0x80808080u, (uint32_t)(j % 4) | (uint32_t)(4 + j % 4) << 16 | 0x0C000C00u);
+                            const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
+                            const f16x2 c = __builtin_bit_cast(f16x2, both | 0x64006400u) - off, d = __builtin_bit_cast(f16x2, d2[x]);
+                            const f16x2 hi = c * d;
+                            f.w[x] = __builtin_bit_cast(uint32_t, hi);
+                            lo.w[x] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, d, -hi));
+                        } else {
+                            const uint32_t u = vr[i][r][j / 2], w = vr[i][r + 1][j / 2];
+                            f.w[x] = j & 1 ? upper_halves(u, w) : lower_halves(u, w);
+                        }
                     }
+                    if constexpr (TYPE == FHIP_Q8_0) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo.h, pp[0].h, acc[j], 0, 0, 0);
 #pragma unroll
                     for (int e = PARTS - 1; e >= 0; e--) {
                         if constexpr (TYPE == FHIP_BF16) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.b, pp[e].b, acc[j], 0, 0, 0);
@@ -840,16 +887,9 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < TILES; i++)
+                for (int r = 0; r < 4; r++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const float d = TYPE == FHIP_Q8_0 ? fhip::kvq_scale(vd[TYPE == FHIP_Q8_0 ? i : 0][r]) : 1.f;
-#pragma unroll
-                        for (int j = 0; j < NJ; j++) {
-                            const float v = TYPE == FHIP_F32 ? __uint_as_float(vr[i][r][j]) : (float)(int8_t)(vr[i][r][j / 4] >> (8 * (j % 4))) * d;
-                            acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, p[i][r], acc[j], 0, 0, 0);
-                        }
-                    }
+                    for (int j = 0; j < NJ; j++) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[0][r][j]), p[0][r], acc[j], 0, 0, 0);
             }
             if constexpr (more()) {
                 load_v(nxt);
@@ -869,9 +909,9 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
             for (uint32_t k = 0; k + 1 < mine; k++) work(k, std::true_type());
             work(mine - 1, std::false_type());
         }
-        if constexpr (TYPE == FHIP_F16) {
+        if constexpr (TYPE == FHIP_F16 || TYPE == FHIP_Q8_0) {
 #pragma unroll
-            for (int j = 0; j < NJ; j++) acc[j] *= 1.f / 32768.f;
+            for (int j = 0; j < NJ; j++) acc[j] *= TYPE == FHIP_F16 ? 1.f / 32768.f : 1.f / 128.f;
         }
 
         // the waves' shares joined; element r of acc[j] is dim dim_of(j, 4 kg + r) of head n

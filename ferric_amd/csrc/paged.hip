@@ -69,10 +69,9 @@ __device__ __forceinline__ uint32_t rows_of(const PagedView& kv, const uint32_t*
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, false)); }
 template <int CTRL>
-__device__ __forceinline__ double dpp(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, false), hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, false);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+__device__ __forceinline__ uint64_t dpp(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xF, 0xF, false), hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, 0xF, 0xF, false);
+    return (uint64_t)hi << 32 | lo;
 }
 // over the 16 lanes of a row, in all of them
 template <typename T, typename Op>
@@ -83,15 +82,63 @@ __device__ __forceinline__ T row16(T v, Op op) {
     return op(v, dpp<0x140>(v));   // row_mirror
 }
 
+// with the other row of a half wave, the other half of the wave: the same in both
+template <typename Op>
+__device__ __forceinline__ float both_rows(float v, Op op) {
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+template <typename Op>
+__device__ __forceinline__ float both_halves(float v, Op op) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+// what the lane 32 lanes away holds (HD = 128), or 16 (64)
+template <int HD>
+__device__ __forceinline__ float across(float v, int lane) {
+    if constexpr (HD == 128) {
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float(lane & 32 ? a[0] : a[1]);
+    } else {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float(lane & 16 ? a[0] : a[1]);
+    }
+}
+
 // ---------------------------------------------------------------- storing the rows of new tokens
 // Row i of the fused projection: + bias, RMS norm of query and key heads, rotation, queries to q_out, keys and values to the row of their page, rounded once.
 // The angle pos * base^(-2c / n_rot) is formed in f64, in turns, and only its fraction of a turn is rounded to f32: the f32 product that the contiguous
 // caches' post-processing forms is 4e-3 rad off at position 100 000.
 // A lane holds two neighbouring dims, so a wave holds 128 values (a slice): one head of 128 or two of 64. TOK tokens a workgroup: with 4 a wave has a
 // token to itself and the f64 work of its angles is shared by all of the token's heads; with 1 the waves share a token's slices.
+// values `at` and `at` + 1 of a pool; for Q8_0 the 16 lanes of a block together: d = amax / 127, codes round(v / d) half away from zero, as fhip_kvq_append's
+template <int TYPE>
+__device__ __forceinline__ void store_pair(const PagedView& kv, bool is_k, size_t at, float2 v, bool placed) {
+    void* pool = is_k ? kv.k : kv.v;
+    if constexpr (TYPE == FHIP_F32) {
+        if (placed) *(float2*)((float*)pool + at) = v;
+    } else if constexpr (TYPE == FHIP_BF16) {
+        if (placed) *(uint32_t*)((uint16_t*)pool + at) = pack_bf16(v.x, v.y);
+    } else if constexpr (TYPE == FHIP_F16) {
+        if (placed) *(uint32_t*)((uint16_t*)pool + at) = pack_f16(v.x, v.y);
+    } else {
+#pragma clang fp contract(off)
+        const float amax = row16(fmaxf(fmaxf(0.f, fabsf(v.x)), fabsf(v.y)), [](float a, float b) { return fmaxf(a, b); });
+        const float d = amax / 127.0f, inv = d > 0.f ? 1.0f / d : 0.f;
+        auto code = [&](float y) {
+            const float t = y * inv, q = copysignf(floorf(fabsf(t) + 0.5f), t);
+            return q != q ? 0 : (int)fminf(fmaxf(q, -127.0f), 127.0f);
+        };
+        if (placed) {
+            *(uint16_t*)((uint8_t*)pool + at) = (uint16_t)((code(v.x) & 255) | (code(v.y) & 255) << 8);
+            if ((threadIdx.x & 15) == 0) (is_k ? kv.k_scales : kv.v_scales)[at >> 5] = __half_as_ushort(__float2half_rn(d));
+        }
+    }
+}
 template <int TYPE, int HD, int TOK>
 __global__ __launch_bounds__(256) void append_kernel(PagedView kv, PagedPost p, int slices_per_wave) {
     constexpr int LPH = HD / 2;                       // lanes of a head
+    constexpr int AHEAD = TOK == 1 ? 1 : 8;           // slices requested together
     __shared__ float2 turns[TOK][HD / 2];             // cos, sin of pair c
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int per_tok = p.n_head + 2 * kv.n_kv, slices = (per_tok * HD + 127) / 128;
@@ -121,7 +168,6 @@ __global__ __launch_bounds__(256) void append_kernel(PagedView kv, PagedPost p, 
     const int j0 = 2 * (lane % LPH);
     float2 t0 = make_float2(1.f, 0.f), t1 = t0;
     int from = lane;                                  // the lane of the partners (split halves)
-    const bool odd = !p.interleaved && (half & 1);    // partners of a lane's two dims in two lanes
     if (j0 < p.n_rot) {
         const float2* turn = turns[TOK == 1 ? 0 : wave];
         if (p.interleaved) {
@@ -136,73 +182,72 @@ __global__ __launch_bounds__(256) void append_kernel(PagedView kv, PagedPost p, 
         }
     }
     const float* x = p.qkv + (size_t)i * per_tok * HD;
-    for (int s = s0; s < s0 + slices_per_wave && s < slices; s++) {
-        const int h = s * (128 / HD) + lane / LPH;    // with heads of 64 the last slice may hold one head only
-        const bool live = h < per_tok;
-        const bool is_q = h < p.n_head, is_k = !is_q && h < p.n_head + kv.n_kv;
-        float2 v = live ? *(const float2*)(x + (size_t)h * HD + j0) : make_float2(0.f, 0.f);
-        if (p.bias && live) {
-            const float2 b = *(const float2*)(p.bias + (size_t)h * HD + j0);
-            v.x += b.x;
-            v.y += b.y;
+    const float2 one = make_float2(1.f, 1.f), wq = p.q_norm ? *(const float2*)(p.q_norm + j0) : one, wk = p.k_norm ? *(const float2*)(p.k_norm + j0) : one;
+    const int s1 = s0 + slices_per_wave < slices ? s0 + slices_per_wave : slices;
+    for (int s = s0; s < s1; s += AHEAD) {
+        float2 v[AHEAD];
+        int head[AHEAD];                              // per_tok and more: none (the last slice of heads of 64 may hold one head only)
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) {
+            head[e] = s + e < s1 ? (s + e) * (128 / HD) + lane / LPH : per_tok;
+            v[e] = head[e] < per_tok ? *(const float2*)(x + (size_t)head[e] * HD + j0) : make_float2(0.f, 0.f);
         }
-        const float* nw = is_q ? p.q_norm : is_k ? p.k_norm : nullptr;
-        float sq = fmaf(v.x, v.x, v.y * v.y);
-        sq = row16(sq, [](float a, float b) { return a + b; });
-        sq += __shfl_xor(sq, 16);
-        if (HD == 128) sq += __shfl_xor(sq, 32);
-        if (nw) {
-            const float inv = 1.0f / sqrtf(sq / (float)HD + p.eps);
-            const float2 w = *(const float2*)(nw + j0);
-            v.x = v.x * inv * w.x;
-            v.y = v.y * inv * w.y;
-        }
-        float2 r = v;
-        if (p.interleaved) {
-            r.x = fmaf(v.x, t0.x, -(v.y * t0.y));
-            r.y = fmaf(v.y, t0.x, v.x * t0.y);
-        } else if (half > 0) {
-            float ox, oy;
-            if (odd) {                                // the partner of dim j is dim j +- half, of the other parity
-                const int d = j0 < half ? half : -half, d1 = j0 + 1 < half ? half : -half, base = lane - lane % LPH;
-                const int f0 = base + (((j0 + d) >> 1) & (LPH - 1)), f1 = base + (((j0 + 1 + d1) >> 1) & (LPH - 1));
-                ox = __shfl(v.y, f0);
-                oy = __shfl(v.x, f1);
-            } else {
-                ox = __shfl(v.x, from);
-                oy = __shfl(v.y, from);
-            }
-            if (j0 < p.n_rot) {
-                r.x = fmaf(v.x, t0.x, -(ox * t0.y));
-                r.y = fmaf(v.y, t1.x, -(oy * t1.y));
+        if (p.bias) {
+            float2 add[AHEAD];
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) add[e] = head[e] < per_tok ? *(const float2*)(p.bias + (size_t)head[e] * HD + j0) : make_float2(0.f, 0.f);
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) {
+                v[e].x += add[e].x;
+                v[e].y += add[e].y;
             }
         }
-        if (is_q || is_k) v = r;
-        if (!live) continue;
-        if (is_q) {
-            *(float2*)(p.q_out + ((size_t)i * p.n_head + h) * HD + j0) = v;
-            continue;
+        if (p.q_norm || p.k_norm) {
+#pragma unroll
+            for (int e = 0; e < AHEAD; e++) {
+                float sq = row16(fmaf(v[e].x, v[e].x, v[e].y * v[e].y), [](float a, float b) { return a + b; });
+                sq = both_rows(sq, [](float a, float b) { return a + b; });
+                if (HD == 128) sq = both_halves(sq, [](float a, float b) { return a + b; });
+                const bool is_q = head[e] < p.n_head, normed = is_q ? p.q_norm != nullptr : head[e] < p.n_head + kv.n_kv && p.k_norm;
+                const float inv = 1.0f / sqrtf(sq / (float)HD + p.eps);
+                if (normed) {
+                    v[e].x = v[e].x * inv * (is_q ? wq.x : wk.x);
+                    v[e].y = v[e].y * inv * (is_q ? wq.y : wk.y);
+                }
+            }
         }
-        const size_t at = (row * kv.n_kv + (h - p.n_head - (is_k ? 0 : kv.n_kv))) * HD + j0;
-        void* pool = is_k ? kv.k : kv.v;
-        if constexpr (TYPE == FHIP_F32) {
-            if (placed) *(float2*)((float*)pool + at) = v;
-        } else if constexpr (TYPE == FHIP_BF16) {
-            if (placed) *(uint32_t*)((uint16_t*)pool + at) = pack_bf16(v.x, v.y);
-        } else if constexpr (TYPE == FHIP_F16) {
-            if (placed) *(uint32_t*)((uint16_t*)pool + at) = pack_f16(v.x, v.y);
-        } else {
-#pragma clang fp contract(off)
-            // a block is the 16 lanes of a row: d = amax / 127, codes round(v / d) half away from zero, as fhip_kvq_append's
-            const float amax = row16(fmaxf(fmaxf(0.f, fabsf(v.x)), fabsf(v.y)), [](float a, float b) { return fmaxf(a, b); });
-            const float d = amax / 127.0f, inv = d > 0.f ? 1.0f / d : 0.f;
-            auto code = [&](float y) {
-                const float t = y * inv, q = copysignf(floorf(fabsf(t) + 0.5f), t);
-                return q != q ? 0 : (int)fminf(fmaxf(q, -127.0f), 127.0f);
-            };
-            if (placed) {
-                *(uint16_t*)((uint8_t*)pool + at) = (uint16_t)((code(v.x) & 255) | (code(v.y) & 255) << 8);
-                if ((lane & 15) == 0) (is_k ? kv.k_scales : kv.v_scales)[at >> 5] = __half_as_ushort(__float2half_rn(d));
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) {
+            float2 r = v[e];
+            if (p.interleaved) {
+                r.x = fmaf(v[e].x, t0.x, -(v[e].y * t0.y));
+                r.y = fmaf(v[e].y, t0.x, v[e].x * t0.y);
+            } else if (half > 0) {
+                float2 o;                             // the partners
+                if (p.n_rot == HD) {                  // half a head away: 32 lanes, or 16
+                    o = make_float2(across<HD>(v[e].x, lane), across<HD>(v[e].y, lane));
+                } else if (half & 1) {                // the partner of dim j is dim j +- half, of the other parity
+                    const int d = j0 < half ? half : -half, d1 = j0 + 1 < half ? half : -half, base = lane - lane % LPH;
+                    o.x = __shfl(v[e].y, base + (((j0 + d) >> 1) & (LPH - 1)));
+                    o.y = __shfl(v[e].x, base + (((j0 + 1 + d1) >> 1) & (LPH - 1)));
+                } else {
+                    o = make_float2(__shfl(v[e].x, from), __shfl(v[e].y, from));
+                }
+                if (j0 < p.n_rot) {
+                    r.x = fmaf(v[e].x, t0.x, -(o.x * t0.y));
+                    r.y = fmaf(v[e].y, t1.x, -(o.y * t1.y));
+                }
+            }
+            if (head[e] < p.n_head + kv.n_kv) v[e] = r;
+        }
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) {
+            const int h = head[e];
+            if (h < p.n_head) {
+                *(float2*)(p.q_out + ((size_t)i * p.n_head + h) * HD + j0) = v[e];
+            } else if (h < per_tok) {
+                const bool is_k = h < p.n_head + kv.n_kv;
+                store_pair<TYPE>(kv, is_k, (row * kv.n_kv + (h - p.n_head - (is_k ? 0 : kv.n_kv))) * HD + j0, v[e], placed);
             }
         }
     }
@@ -260,36 +305,86 @@ __device__ __forceinline__ uint64_t order_key(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     return b >> 63 ? ~b : b | 1ull << 63;
 }
+// On v_mfma_f64_16x16x4_f64: 16 pages by the head's queries, max(q, 0) and min(q, 0) in f64 in registers, a lane's bounds four neighbouring dims of a page at a time. Bound by the
+// bounds' bytes: the instructions of 16 pages take 4096 cycles, 9.8 TB/s of bounds on the chip. A wave a page, with a sum over its lanes for each query, took 75 us of 24 sequences of 4 KV heads of 8, 52 MB.
 template <int HD>
-__global__ __launch_bounds__(256) void score_kernel(PagedView kv, const float* __restrict__ q, const uint32_t* __restrict__ lens, uint32_t max_len, const float* __restrict__ bounds,
-                                                    int n_head, uint32_t first, uint32_t last, uint64_t* __restrict__ keys, uint32_t key_stride) {
-    const int lane = threadIdx.x & 63, g = n_head / kv.n_kv, head = blockIdx.y;
-    const uint32_t seq = blockIdx.z, pages = pages_of(kv, rows_of(kv, lens, seq, max_len));
-    const uint32_t j = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (j >= pages) return;
-    const uint32_t page = kv.table[seq * kv.table_stride + j];
-    double best = -INFINITY;
-    if (page < kv.n_pages) {
-        const float* b = bounds + ((size_t)page * kv.n_kv + head) * 2 * HD;
-        for (int e = 0; e < g; e++) {
-            double s = 0;
-            for (int d = lane; d < HD; d += 64) {
-                const double x = q[((size_t)seq * n_head + head * g + e) * HD + d], u = x * (double)b[d], w = x * (double)b[HD + d];
-                s += u > w || u != u ? u : w;
-            }
-            for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-            best = s > best || s != s ? s : best;
+__global__ __launch_bounds__(256, 2) void score_kernel(PagedView kv, const float* __restrict__ q, const uint32_t* __restrict__ lens, uint32_t max_len, const float* __restrict__ bounds,
+                                                       int n_head, uint32_t first, uint32_t last, uint64_t* __restrict__ keys, uint32_t key_stride) {
+    constexpr int NI = HD / 16;
+    const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4, g = n_head / kv.n_kv, head = blockIdx.y;
+    const uint32_t seq = blockIdx.z, pages = pages_of(kv, rows_of(kv, lens, seq, max_len)), groups = (pages + 15) / 16;
+    uint32_t j = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (j >= groups) return;
+    const uint32_t* table = kv.table + seq * kv.table_stride;
+    keys += ((size_t)seq * kv.n_kv + head) * key_stride;
+    double up[NI][4], down[NI][4];
+    const float* qh = q + ((size_t)seq * n_head + head * g + (n < g ? n : 0)) * HD + 4 * kg;
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const f32x4 x = *(const f32x4*)(qh + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            up[i][e] = x[e] > 0.f || x[e] != x[e] ? (double)x[e] : 0.0;
+            down[i][e] = x[e] < 0.f ? (double)x[e] : 0.0;
         }
     }
-    if (lane == 0) keys[((size_t)seq * kv.n_kv + head) * key_stride + j] = j < first || j + last >= pages ? ~0ull : order_key(best);
+    for (; j < groups; j += gridDim.x * 4) {
+        const uint32_t mine = 16 * j + n < pages ? table[16 * j + n] : NO_PAGE;
+        const float* b = bounds + ((size_t)(mine < kv.n_pages ? mine : 0) * kv.n_kv + head) * 2 * HD + 4 * kg;
+        f32x4 lo[NI], hi[NI];
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            lo[i] = *(const f32x4*)(b + 16 * i);
+            hi[i] = *(const f32x4*)(b + HD + 16 * i);
+        }
+        f64x4 s = (f64x4){0, 0, 0, 0}, s2 = s;
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s = __builtin_amdgcn_mfma_f64_16x16x4f64((double)hi[i][e], up[i][e], s, 0, 0, 0);
+                s2 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)lo[i][e], down[i][e], s2, 0, 0, 0);
+            }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {                 // page 16 j + 4 r + kg, query n
+            const uint32_t page = 16 * j + 4 * r + kg;
+            const bool there = __shfl(mine, 4 * r + kg) < kv.n_pages;
+            uint64_t key = n < g && there ? order_key(s[r] + s2[r]) : order_key(-INFINITY);
+            key = row16(key, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+            if (n == 0 && page < pages) keys[page] = page < first || page + last >= pages ? ~0ull : key;
+        }
+    }
 }
 
 // The n_select largest keys of a list, equal ones by their place, as ascending places. One workgroup a list. The key that the last chosen one has is found by counting: the
 // interval that holds it is cut into 1024 by its width, and the one of these with it is the next interval.
-constexpr int SEL_T = 512, SEL_BINS = 1024;
+constexpr int SEL_T = 1024, SEL_BINS = 1024, SEL_HELD = 8;
+// Over the workgroup: each thread's sum of those in front of it, and of all. buf: a word for each wave.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* buf, int lane, int wave, uint32_t& all) {
+    uint32_t upto = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t t = __shfl_up(upto, o);
+        if (lane >= o) upto += t;
+    }
+    __syncthreads();
+    if (lane == 63) buf[wave] = upto;
+    __syncthreads();
+    uint32_t before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < SEL_T / 64; w++) {
+        const uint32_t c = buf[w];
+        before += w < wave ? c : 0;
+        total += c;
+    }
+    all = total;
+    return before + upto - v;
+}
+// HELD: the keys stay in registers, SEL_HELD neighbouring ones a thread; otherwise (more than SEL_T * SEL_HELD) they are read again for each pass.
+template <bool HELD>
 __global__ __launch_bounds__(SEL_T) void select_kernel(PagedView kv, const uint32_t* __restrict__ lens, uint32_t max_len, uint32_t n_select, const uint64_t* __restrict__ keys,
                                                        uint32_t key_stride, uint32_t kept, uint32_t* __restrict__ out) {
-    __shared__ uint32_t hist[SEL_BINS], counts[2][SEL_T / 64];
+    __shared__ uint32_t hist[SEL_BINS], buf[SEL_T / 64];
     __shared__ uint64_t edge[2][SEL_T / 64];
     __shared__ uint32_t found[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -301,84 +396,89 @@ __global__ __launch_bounds__(SEL_T) void select_kernel(PagedView kv, const uint3
         for (uint32_t j = tid; j < n_select; j += SEL_T) out[j] = j < n ? j : NO_PAGE;
         return;
     }
+    uint64_t held[SEL_HELD];
+    if (HELD)
+#pragma unroll
+        for (int e = 0; e < SEL_HELD; e++) held[e] = tid * SEL_HELD + e < n ? keys[tid * SEL_HELD + e] : 0;
+    // f(key, place) of this thread's keys, in their order where HELD
+    auto each = [&](auto f) {
+        if constexpr (HELD) {
+#pragma unroll
+            for (int e = 0; e < SEL_HELD; e++)
+                if (tid * SEL_HELD + e < n) f(held[e], (uint32_t)(tid * SEL_HELD + e));
+        } else {
+            for (uint32_t j = tid; j < n; j += SEL_T) f(keys[j], j);
+        }
+    };
     uint64_t lo = ~0ull, hi = 0;
-    for (uint32_t j = tid; j < n; j += SEL_T) {
-        const uint64_t k = keys[j];
-        if (k == ~0ull) continue;                     // kept whatever its score
+    each([&](uint64_t k, uint32_t) {
+        if (k == ~0ull) return;                       // kept whatever its score
         lo = k < lo ? k : lo;
         hi = k > hi ? k : hi;
-    }
+    });
+#pragma unroll
     for (int o = 32; o; o >>= 1) {
         const uint64_t a = __shfl_xor((unsigned long long)lo, o), b = __shfl_xor((unsigned long long)hi, o);
         lo = a < lo ? a : lo;
         hi = b > hi ? b : hi;
     }
     if (lane == 0) { edge[0][wave] = lo; edge[1][wave] = hi; }
+    hist[tid] = 0;
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < SEL_T / 64; w++) {
         lo = edge[0][w] < lo ? edge[0][w] : lo;
         hi = edge[1][w] > hi ? edge[1][w] : hi;
     }
     uint32_t want = n_select - kept;                  // of the keys within [lo, hi], the largest `want` are chosen; here n > n_select >= kept, so it holds some
-    while (want > 0 && lo < hi) {
-        const int shift = 64 - __builtin_clzll(hi - lo) > 10 ? 64 - __builtin_clzll(hi - lo) - 10 : 0;      // (hi - lo) >> shift < 1024
-        for (int b = tid; b < SEL_BINS; b += SEL_T) hist[b] = 0;
-        __syncthreads();
-        for (uint32_t j = tid; j < n; j += SEL_T) {
-            const uint64_t k = keys[j];
+    while (want > 0 && lo < hi) {                     // (hist is clear here)
+        const int bits = 64 - __builtin_clzll(hi - lo), shift = bits > 10 ? bits - 10 : 0;      // (hi - lo) >> shift < 1024
+        each([&](uint64_t k, uint32_t) {
             if (k >= lo && k <= hi) atomicAdd(&hist[(uint32_t)((k - lo) >> shift)], 1u);
-        }
+        });
         __syncthreads();
-        if (wave == 0) {                              // a lane has 16 bins, the highest first
-            uint32_t mine = 0;
-            for (int b = 0; b < 16; b++) mine += hist[SEL_BINS - 1 - (16 * lane + b)];
-            uint32_t upto = mine;
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t t = __shfl_up(upto, o);
-                if (lane >= o) upto += t;
-            }
-            uint32_t above = upto - mine;
-            if (above < want && upto >= want)
-                for (int b = 0; b < 16; b++) {
-                    const int bin = SEL_BINS - 1 - (16 * lane + b);
-                    const uint32_t c = hist[bin];
-                    if (above < want && above + c >= want) {
-                        found[0] = (uint32_t)bin;
-                        found[1] = want - above;
-                    }
-                    above += c;
-                }
+        const uint32_t mine = hist[SEL_BINS - 1 - tid];      // the highest bin first
+        uint32_t all;
+        const uint32_t above = block_scan(mine, buf, lane, wave, all);
+        if (above < want && above + mine >= want) {
+            found[0] = SEL_BINS - 1 - tid;
+            found[1] = want - above;
         }
+        hist[SEL_BINS - 1 - tid] = 0;
         __syncthreads();
         const uint64_t bin = found[0];
         if (bin < (hi - lo) >> shift) hi = lo + ((bin + 1) << shift) - 1;
         lo += bin << shift;
         want = found[1];
-        __syncthreads();
     }
     // places of the keys above it, and of the first `want` that equal it
-    uint32_t done = 0, equal = 0;
-    for (uint32_t j0 = 0; j0 < n; j0 += SEL_T) {
-        const uint32_t j = j0 + tid;
-        const uint64_t k = j < n ? keys[j] : 0;
-        const bool same = j < n && k == lo && k != ~0ull;
-        const uint64_t below = ((uint64_t)1 << lane) - 1, same_mask = __ballot(same);
-        if (lane == 0) counts[0][wave] = __popcll(same_mask);
-        __syncthreads();
-        uint32_t rank = equal + __popcll(same_mask & below);
-        for (int w = 0; w < wave; w++) rank += counts[0][w];
-        const bool take = (j < n && (k == ~0ull || (want > 0 && k > lo))) || (same && rank < want);
-        const uint64_t take_mask = __ballot(take);
-        if (lane == 0) counts[1][wave] = __popcll(take_mask);
-        __syncthreads();
-        uint32_t at = done + __popcll(take_mask & below);
-        for (int w = 0; w < wave; w++) at += counts[1][w];
-        if (take) out[at] = j;
-        for (int w = 0; w < SEL_T / 64; w++) {
-            equal += counts[0][w];
-            done += counts[1][w];
+    auto above = [&](uint64_t k) { return k == ~0ull || (want > 0 && k > lo); };
+    auto equal = [&](uint64_t k) { return k == lo && k != ~0ull; };
+    uint32_t all;
+    if constexpr (HELD) {
+        uint32_t same = 0, take = 0;
+        each([&](uint64_t k, uint32_t) { same += equal(k); });
+        uint32_t rank = block_scan(same, buf, lane, wave, all);
+        const uint32_t rank0 = rank;
+        each([&](uint64_t k, uint32_t) { take += above(k) || (equal(k) && rank++ < want); });
+        uint32_t at = block_scan(take, buf, lane, wave, all);
+        rank = rank0;
+        each([&](uint64_t k, uint32_t j) {
+            if (above(k) || (equal(k) && rank++ < want)) out[at++] = j;
+        });
+    } else {
+        uint32_t done = 0, ties = 0;
+        for (uint32_t j0 = 0; j0 < n; j0 += SEL_T) {
+            const uint32_t j = j0 + tid;
+            const uint64_t k = j < n ? keys[j] : 0;
+            const bool same = j < n && equal(k);
+            const uint32_t rank = ties + block_scan(same, buf, lane, wave, all);
+            ties += all;
+            const bool take = j < n && (above(k) || (same && rank < want));
+            const uint32_t at = done + block_scan(take, buf, lane, wave, all);
+            done += all;
+            if (take) out[at] = j;
         }
-        __syncthreads();
     }
 }
 
@@ -415,10 +515,8 @@ __device__ __forceinline__ uint32_t upper_halves(uint32_t a, uint32_t b) { retur
 __device__ __forceinline__ uint32_t lower_halves(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 // the largest of a column's four lanes, in all of them
 __device__ __forceinline__ float column_max(float v) {
-    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+    auto larger = [](float a, float b) { return fmaxf(a, b); };
+    return both_rows(both_halves(v, larger), larger);
 }
 // Two codes of a Q8_0 block as f16: byte c + 128 in the bits of 1024 + c + 128, less 1152. sel: 0x04ii04jj for bytes j and i.
 __device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t sel) {
@@ -1080,11 +1178,13 @@ int launch_paged_select(int hd, const PagedView& kv, const float* q, const uint3
                         uint32_t first, uint32_t last, void* ws, uint32_t* out, hipStream_t s) {
     const uint32_t pages = pages_at_most(kv, max_len);
     if (pages > 0) {
-        const dim3 grid((pages + 3) / 4, kv.n_kv, kv.n_seq);
+        const dim3 grid((pages + 63) / 64, kv.n_kv, kv.n_seq);
         if (hd == 128) hipLaunchKernelGGL((score_kernel<128>), grid, dim3(256), 0, s, kv, q, lens, max_len, bounds, n_head, first, last, (uint64_t*)ws, pages);
         else hipLaunchKernelGGL((score_kernel<64>), grid, dim3(256), 0, s, kv, q, lens, max_len, bounds, n_head, first, last, (uint64_t*)ws, pages);
     }
-    hipLaunchKernelGGL(select_kernel, dim3(kv.n_seq * kv.n_kv), dim3(SEL_T), 0, s, kv, lens, max_len, n_select, (const uint64_t*)ws, pages, first + last, out);
+    const dim3 lists(kv.n_seq * kv.n_kv);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, lists, dim3(SEL_T), 0, s, kv, lens, max_len, n_select, (const uint64_t*)ws, pages, first + last, out); };
+    pages <= SEL_T * SEL_HELD ? go(select_kernel<true>) : go(select_kernel<false>);
     return check_hip(hipGetLastError(), "paged_select launch");
 }
 

@@ -1745,7 +1745,7 @@ int fhip_paged_append(const fhip_paged* kv, const float* d_qkv, const float* d_b
 size_t fhip_paged_attention_ws_bytes(const fhip_paged* kv, size_t n_head, size_t max_len) {
     fhip::PagedView v;
     if (paged_view("fhip_paged_attention_ws_bytes", kv, v) || paged_heads("fhip_paged_attention_ws_bytes", kv, n_head)) return 0;
-    return fhip::paged_attention_ws_bytes(v, (int)kv->head_dim, (int)n_head, paged_bound(max_len));
+    return fhip::paged_attention_ws_bytes(kv->type, v, (int)kv->head_dim, (int)n_head, paged_bound(max_len));
 }
 static int paged_attention(const char* who, const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, size_t max_len, const uint32_t* d_selected, size_t n_select,
                            size_t n_head, size_t window, float softcap, float* d_ws, float* d_out, void* stream) {
@@ -1758,7 +1758,7 @@ static int paged_attention(const char* who, const fhip_paged* kv, const float* d
     if (!aligned16(d_q) || !aligned16(d_out) || !aligned16(d_ws)) return set_error(FHIP_ERR_ARG, "%s: pointers must be 16-byte aligned", who);
     if ((rc = need_init())) return rc;
     const uint32_t bound = paged_bound(max_len);
-    if (!d_ws && fhip::paged_attention_ws_bytes(v, (int)kv->head_dim, (int)n_head, d_selected ? paged_bound(n_select * kv->page_rows) : bound) > 0)
+    if (!d_ws && fhip::paged_attention_ws_bytes(kv->type, v, (int)kv->head_dim, (int)n_head, d_selected ? paged_bound(n_select * kv->page_rows) : bound) > 0)
         return set_error(FHIP_ERR_ARG, "%s: this call needs a workspace (fhip_paged_attention_ws_bytes)", who);
     return fhip::launch_paged_attention(kv->type, (int)kv->head_dim, v, d_q, d_lens, bound, d_selected, (uint32_t)n_select, (int)n_head, paged_bound(window), softcap, d_ws,
                                         d_out, (hipStream_t)stream);

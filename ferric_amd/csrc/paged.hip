@@ -20,6 +20,8 @@ using fhip::PagedView;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef double f64x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t NO_PAGE = 0xFFFFFFFFu;
 
@@ -614,6 +616,7 @@ struct Attend {
     const uint32_t* lens;
     const uint32_t* selected;
     float *out, *part;      // part: per workgroup two times g rows of HD, then g (maximum, sum), and 2 g words to keep the next one aligned
+    uint32_t* plan;         // per unit: the first and the last workgroup with steps of it, and whether it is the first one's second share; first = last: nothing to join
     uint32_t max_len, n_select, window;
     int n_head;
     float softcap, scale;
@@ -621,16 +624,20 @@ struct Attend {
     uint32_t min_steps;
 };
 
+// What a unit costs in steps beside its own: its queries, its first keys' trip and the waves' sums. Without it a workgroup that has many short sequences' units was the last by far: 24 sequences
+// of 1 .. 4096 keys on bf16 took 58 us where as many keys in sequences of equal length took 44.
+constexpr uint32_t UNIT_COST = 6;
+__device__ __forceinline__ uint64_t unit_cost(uint32_t steps) { return steps ? (uint64_t)steps + UNIT_COST : 0; }
 // Range of steps of a workgroup: all steps over the workgroups, `least` at least.
-__device__ __forceinline__ uint64_t steps_each(uint64_t all, int log_wgs, uint32_t least) {
+__device__ __forceinline__ uint64_t places_each(uint64_t all, int log_wgs, uint32_t least) {
     const uint64_t per = (all + ((uint64_t)1 << log_wgs) - 1) >> log_wgs;
     return per > least ? per : least;
 }
 template <int TYPE, bool SEL>
-__device__ __forceinline__ uint64_t all_steps(const Attend& a, int lane) {
+__device__ __forceinline__ uint64_t all_places(const Attend& a, int lane) {
     uint64_t all = 0;
     for (uint32_t b = 0; b < a.kv.n_seq; b += 64) {
-        const uint64_t c = b + lane < a.kv.n_seq ? (uint64_t)span_of<TYPE, SEL>(a.kv, a.lens, b + lane, a.max_len, a.window, a.n_select).steps * a.kv.n_kv : 0;
+        const uint64_t c = b + lane < a.kv.n_seq ? unit_cost(span_of<TYPE, SEL>(a.kv, a.lens, b + lane, a.max_len, a.window, a.n_select).steps) * a.kv.n_kv : 0;
         all += __shfl((unsigned long long)wave_scan(c, lane), 63);
     }
     return all;
@@ -648,40 +655,46 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
     const int g = a.n_head / kv.n_kv;
 
     // this workgroup's steps, and the unit that the first of them belongs to
-    uint64_t at = 0, end = ~0ull, unit0 = 0;          // unit0: the first step of sequence `seq`
-    uint32_t seq = 0, head = 0, from = 0;
+    uint64_t at = 0, end = ~0ull, unit0 = 0, each = 1;      // places [at, end) of the row of all units; unit0: the current unit's first
+    uint32_t seq = 0, head = 0, shares = 0;
     Span sp;
     if (a.log_wgs < 0) {
         seq = blockIdx.x / kv.n_kv;
         head = blockIdx.x % kv.n_kv;
         sp = uniform(span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select));
     } else {
-        const uint64_t all = uniform(all_steps<TYPE, SEL>(a, lane)), per = steps_each(all, a.log_wgs, a.min_steps);
+        const uint64_t all = uniform(all_places<TYPE, SEL>(a, lane)), per = places_each(all, a.log_wgs, a.min_steps);
         at = blockIdx.x * per;
         end = at + per < all ? at + per : all;
         if (at >= end) return;
         uint64_t before = 0;
         for (uint32_t b = 0; b < kv.n_seq; b += 64) {
-            const uint64_t c = b + lane < kv.n_seq ? (uint64_t)span_of<TYPE, SEL>(kv, a.lens, b + lane, a.max_len, a.window, a.n_select).steps * kv.n_kv : 0;
+            const uint64_t c = b + lane < kv.n_seq ? unit_cost(span_of<TYPE, SEL>(kv, a.lens, b + lane, a.max_len, a.window, a.n_select).steps) * kv.n_kv : 0;
             const uint64_t upto = before + wave_scan(c, lane), here = __ballot(upto > at);
             if (here) {
                 const int l = __builtin_ctzll(here);
                 seq = b + l;
-                unit0 = __shfl((unsigned long long)(upto - c), l);
+                before = __shfl((unsigned long long)(upto - c), l);
                 break;
             }
             before = __shfl((unsigned long long)upto, 63);
         }
         seq = uniform(seq);
-        unit0 = uniform(unit0);
+        before = uniform(before);
         sp = uniform(span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select));
-        head = uniform((uint32_t)((at - unit0) / sp.steps));
-        from = uniform((uint32_t)((at - unit0) - (uint64_t)head * sp.steps));
+        // a unit's first UNIT_COST places in the row are no steps
+        const uint64_t cost = unit_cost(sp.steps);
+        head = uniform((uint32_t)((at - before) / cost));
+        unit0 = before + head * cost;
+        each = per;
     }
-    const uint64_t range0 = at;
 
     for (;;) {
-        const uint32_t to = a.log_wgs < 0 || end - at > sp.steps - from ? sp.steps : from + (uint32_t)(end - at);   // steps [from, to) of the unit
+        // steps [from, to) of the unit are this workgroup's: those of the places [at, end)
+        auto step_at = [&](uint64_t place) { return place <= unit0 + UNIT_COST ? 0u : place - unit0 - UNIT_COST < sp.steps ? (uint32_t)(place - unit0 - UNIT_COST) : sp.steps; };
+        const uint32_t from = step_at(at), to = a.log_wgs < 0 ? sp.steps : step_at(end);
+        const bool whole = from == 0 && to == sp.steps;
+        if (to > from || a.log_wgs < 0) {
         const uint32_t* table = kv.table + seq * kv.table_stride;
         const uint32_t* list = SEL ? a.selected + ((size_t)seq * kv.n_kv + head) * a.n_select : nullptr;
         const uint32_t pages = pages_of(kv, sp.len), row_values = (uint32_t)kv.n_kv * HD;
@@ -729,60 +742,73 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
         uint32_t kr[TILES][KW * 4], vr[TILES][4][VW];
         uint32_t kd[TYPE == FHIP_Q8_0 ? TILES : 1][4][NB / 2];      // two scales a word
         uint16_t vd[TYPE == FHIP_Q8_0 ? TILES : 1][4];
-        const uint32_t k_off = (uint32_t)(n * row_values * Elem<TYPE>::BYTES) + (TYPE == FHIP_Q8_0 ? 8 : 16) * kg;
-        // (the parts of both tiles in turn, as the products take them)
+        const uint32_t k_off = n * row_values * Elem<TYPE>::BYTES + (TYPE == FHIP_Q8_0 ? 8 : 16) * kg;      // of a lane's parts from their tile's first byte
+        uint32_t v_off[4], d_off[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            v_off[r] = (4 * kg + r) * row_values * Elem<TYPE>::BYTES + (TYPE == FHIP_F32 ? 16 : VB) * n;
+            d_off[r] = (4 * kg + r) * (row_values / 16);
+        }
+        // A tile's bytes from the KV head's first on, as a buffer: the address in scalar registers and a lane's 32-bit offset from it, where a pointer's loads cost an addition of
+        // 64 bits a lane each, a tenth of a Q8_0 step's instructions.
+        auto tile_bytes = [&](const void* pool, uint64_t bytes) { return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)pool + bytes), 0, (int)(16 * row_values * 4), 0x00027000); };
         auto load_k = [&](const Tile (&t)[TILES]) {
             if constexpr (TYPE == FHIP_Q8_0) {
 #pragma unroll
-                for (int i = 0; i < TILES; i++)
+                for (int i = 0; i < TILES; i++) {
+                    const auto scales = tile_bytes(kv.k_scales, t[i].at >> 5 << 1), base = tile_bytes(kv.k, t[i].at);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const uint16_t* s = kv.k_scales + (t[i].at >> 5) + (uint32_t)(4 * kg + r) * (row_values / 32);
                         if constexpr (NB == 4) {
-                            const uint2 w = *(const uint2*)s;
+                            const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(scales, d_off[r], 0, 0);
                             kd[i][r][0] = w.x; kd[i][r][1] = w.y;
                         } else {
-                            kd[i][r][0] = *(const uint32_t*)s;
+                            kd[i][r][0] = __builtin_amdgcn_raw_buffer_load_b32(scales, d_off[r], 0, 0);
                         }
                     }
-            }
 #pragma unroll
-            for (int b = 0; b < (TYPE == FHIP_Q8_0 ? NB : KW); b++)
-#pragma unroll
-                for (int i = 0; i < TILES; i++) {
-                    const char* base = (const char*)kv.k + t[i].at * Elem<TYPE>::BYTES + k_off;
-                    if constexpr (TYPE == FHIP_Q8_0) {
-                        const uint2 w = *(const uint2*)(base + 32 * b);
+                    for (int b = 0; b < NB; b++) {
+                        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(base, k_off + 32 * b, 0, 0);
                         kr[i][2 * b] = w.x; kr[i][2 * b + 1] = w.y;
-                    } else {
-                        const uint4 w = *(const uint4*)(base + 64 * b);
-                        kr[i][4 * b] = w.x; kr[i][4 * b + 1] = w.y; kr[i][4 * b + 2] = w.z; kr[i][4 * b + 3] = w.w;
                     }
                 }
+            } else {
+                // (the parts of both tiles in turn, as the products take them)
+                __amdgpu_buffer_rsrc_t base[TILES];
+#pragma unroll
+                for (int i = 0; i < TILES; i++) base[i] = tile_bytes(kv.k, t[i].at * Elem<TYPE>::BYTES);
+#pragma unroll
+                for (int b = 0; b < KW; b++)
+#pragma unroll
+                    for (int i = 0; i < TILES; i++) {
+                        const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(base[i], k_off + 64 * b, 0, 0);
+                        kr[i][4 * b] = w.x; kr[i][4 * b + 1] = w.y; kr[i][4 * b + 2] = w.z; kr[i][4 * b + 3] = w.w;
+                    }
+            }
         };
         auto load_v = [&](const Tile (&t)[TILES]) {
 #pragma unroll
             for (int i = 0; i < TILES; i++) {
-                const char* base = (const char*)kv.v + t[i].at * Elem<TYPE>::BYTES;
+                const auto base = tile_bytes(kv.v, t[i].at * Elem<TYPE>::BYTES);
+                const auto scales = tile_bytes(TYPE == FHIP_Q8_0 ? (const void*)kv.v_scales : kv.v, t[i].at >> 5 << 1);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const uint32_t off = (4 * kg + r) * row_values * Elem<TYPE>::BYTES;
                     if constexpr (TYPE == FHIP_F32) {
 #pragma unroll
                         for (int h = 0; h < HD / 64; h++) {
-                            const uint4 w = *(const uint4*)(base + off + 256 * h + 16 * n);
+                            const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(base, v_off[r] + 256 * h, 0, 0);
                             vr[i][r][4 * h] = w.x; vr[i][r][4 * h + 1] = w.y; vr[i][r][4 * h + 2] = w.z; vr[i][r][4 * h + 3] = w.w;
                         }
                     } else if constexpr (VB == 16) {
-                        const uint4 w = *(const uint4*)(base + off + 16 * n);
+                        const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(base, v_off[r], 0, 0);
                         vr[i][r][0] = w.x; vr[i][r][1] = w.y; vr[i][r][2] = w.z; vr[i][r][3] = w.w;
                     } else if constexpr (VB == 8) {
-                        const uint2 w = *(const uint2*)(base + off + 8 * n);
+                        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(base, v_off[r], 0, 0);
                         vr[i][r][0] = w.x; vr[i][r][1] = w.y;
                     } else {
-                        vr[i][r][0] = *(const uint32_t*)(base + off + 4 * n);
+                        vr[i][r][0] = __builtin_amdgcn_raw_buffer_load_b32(base, v_off[r], 0, 0);
                     }
-                    if constexpr (TYPE == FHIP_Q8_0) vd[i][r] = kv.v_scales[(t[i].at >> 5) + (uint32_t)(4 * kg + r) * (row_values / 32) + n / (16 / NB)];
+                    if constexpr (TYPE == FHIP_Q8_0) vd[i][r] = __builtin_amdgcn_raw_buffer_load_b16(scales, d_off[r] + 2 * (n / (16 / NB)), 0, 0);
                 }
             }
         };
@@ -846,9 +872,9 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                 s[0] += s2;
             } else if constexpr (TYPE == FHIP_Q8_0) {
 #pragma unroll
-                for (int b = 0; b < NB; b++)
+                for (int i = 0; i < TILES; i++)
 #pragma unroll
-                    for (int i = 0; i < TILES; i++) {
+                    for (int b = 0; b < NB; b++) {
                         Frag f;                       // eight codes
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
@@ -903,9 +929,10 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                         const uint32_t key = cur[i].pos + 4 * kg + r;
                         if (cur[i].pos == NO_PAGE || key >= sp.len || key < sp.lo) {
                             s[i][r] = -INFINITY;
+                            if constexpr (TYPE == FHIP_Q8_0) vd[i][r] = 0;      // (codes are numbers whatever lies there)
+                            else
 #pragma unroll
-                            for (int e = 0; e < VW; e++) vr[i][r][e] = 0;
-                            if (TYPE == FHIP_Q8_0) vd[TYPE == FHIP_Q8_0 ? i : 0][r] = 0;
+                                for (int e = 0; e < VW; e++) vr[i][r][e] = 0;
                         }
                     }
                 }
@@ -1024,8 +1051,12 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                 *(f32x4*)&sm_o[wave][n][d] = (f32x4){acc[j][r], acc[j + 1][r], acc[j + 2][r], acc[j + 3][r]};
             }
         __syncthreads();
-        const bool whole = from == 0 && to == sp.steps;
-        float* part = whole ? nullptr : a.part + ((size_t)blockIdx.x * 2 + (at == range0 ? 0 : 1)) * g * (HD + 4);
+        float* part = whole ? nullptr : a.part + ((size_t)blockIdx.x * 2 + shares) * g * (HD + 4);
+        if (a.log_wgs >= 0 && from == 0 && threadIdx.x == 0) {       // the unit's first steps are here: who has the others
+            const uint32_t last = whole ? blockIdx.x : (uint32_t)((unit0 + unit_cost(sp.steps) - 1) / each);
+            a.plan[seq * kv.n_kv + head] = (uint32_t)blockIdx.x | last << 15 | shares << 30;
+        }
+        shares += !whole;
         for (int e = threadIdx.x; e < g * (HD / 4); e += 64 * WV) {
             const int h = e / (HD / 4), d = 4 * (e % (HD / 4));
             float top = sm_m[0][h], sum = 0.f;
@@ -1047,11 +1078,12 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                 if (d == 0) { part[g * HD + 2 * h] = top; part[g * HD + 2 * h + 1] = sum; }
             }
         }
+        }
         if (a.log_wgs < 0) return;
-        at += to - from;
-        if (at >= end) return;
         // the next unit: the sequence's next KV head, or the next sequence with any steps
-        from = 0;
+        unit0 += unit_cost(sp.steps);
+        at = unit0;
+        if (at + UNIT_COST >= end) return;
         if (++head == (uint32_t)kv.n_kv) {
             head = 0;
             do {
@@ -1067,57 +1099,49 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
 template <int TYPE, int HD, bool SEL>
 __global__ __launch_bounds__(256) void join_kernel(Attend a) {
     constexpr int LANES = HD / 4, GROUPS = 256 / LANES;
-    __shared__ float sm_top[4], sm_l[GROUPS];
+    __shared__ float sm_m[GROUPS], sm_l[GROUPS];
     __shared__ __attribute__((aligned(16))) float sm_o[GROUPS][HD];
     const PagedView& kv = a.kv;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = a.n_head / kv.n_kv;
+    const int g = a.n_head / kv.n_kv;
     const uint32_t seq = blockIdx.x / a.n_head, qh = blockIdx.x % a.n_head, head = qh / g, h = qh % g;
-    uint64_t all = 0, before = 0;
-    for (uint32_t b = 0; b < kv.n_seq; b += 64) {
-        const uint64_t c = b + lane < kv.n_seq ? (uint64_t)span_of<TYPE, SEL>(kv, a.lens, b + lane, a.max_len, a.window, a.n_select).steps * kv.n_kv : 0;
-        const uint64_t upto = wave_scan(c, lane);
-        if (seq >= b && seq < b + 64) before = all + __shfl((unsigned long long)(upto - c), seq - b);
-        all += __shfl((unsigned long long)upto, 63);
-    }
-    const uint64_t per = steps_each(all, a.log_wgs, a.min_steps);
+    const uint32_t plan = a.plan[seq * kv.n_kv + head];      // (of nobody's making for a unit without steps)
     const Span sp = span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select);
     float* out = a.out + ((size_t)seq * a.n_head + qh) * HD;
     if (sp.steps == 0) {
         if (threadIdx.x < HD) out[threadIdx.x] = 0.f;
         return;
     }
-    const uint64_t u0 = before + (uint64_t)head * sp.steps, u1 = u0 + sp.steps;
-    const uint32_t w0 = (uint32_t)(u0 / per), w1 = (uint32_t)((u1 - 1) / per);
-    if (w0 == w1) return;                             // the unit lies within one range: finished there
-    auto part = [&](uint32_t w) { return a.part + ((size_t)w * 2 + (w == w0 && u0 > w * per ? 1 : 0)) * g * (HD + 4); };
-    float top = -INFINITY;
-    for (uint32_t w = w0 + threadIdx.x; w <= w1; w += 256) top = fmaxf(top, part(w)[g * HD + 2 * h]);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if (lane == 0) sm_top[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(sm_top[0], sm_top[1]), fmaxf(sm_top[2], sm_top[3]));
-    const float base = top == -INFINITY ? 0.f : top;
+    const uint32_t w0 = plan & 0x7FFFu, w1 = plan >> 15 & 0x7FFFu, second = plan >> 30;
+    if (w0 == w1) return;                             // finished where it was
+    auto part = [&](uint32_t w) { return a.part + ((size_t)w * 2 + (w == w0 ? second : 0)) * g * (HD + 4); };
+    // a group of threads takes every GROUPS-th share; its maximum as it goes
     const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
     f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
+    float top = -INFINITY, sum = 0.f;
     for (uint32_t w = w0 + group; w <= w1; w += GROUPS) {
         const float* p = part(w);
-        const float f = __builtin_amdgcn_exp2f(p[g * HD + 2 * h] - base);
-        sum = fmaf(p[g * HD + 2 * h + 1], f, sum);
-        o += *(const f32x4*)(p + h * HD + d) * f;
+        const float m = p[g * HD + 2 * h], l = p[g * HD + 2 * h + 1];
+        const f32x4 v = *(const f32x4*)(p + h * HD + d);
+        const float now = fmaxf(top, m), base = now == -INFINITY ? 0.f : now, f0 = __builtin_amdgcn_exp2f(top - base), f1 = __builtin_amdgcn_exp2f(m - base);
+        o = o * f0 + v * f1;
+        sum = fmaf(l, f1, sum * f0);
+        top = now;
     }
     *(f32x4*)&sm_o[group][d] = o;
-    if (d == 0) sm_l[group] = sum;
+    if (d == 0) { sm_m[group] = top; sm_l[group] = sum; }
     __syncthreads();
     if (threadIdx.x < HD) {
-        float v = 0.f, t = 0.f;
+        float all = sm_m[0], v = 0.f, t = 0.f;
+#pragma unroll
+        for (int i = 1; i < GROUPS; i++) all = fmaxf(all, sm_m[i]);
+        const float base = all == -INFINITY ? 0.f : all;
 #pragma unroll
         for (int i = 0; i < GROUPS; i++) {
-            v += sm_o[i][threadIdx.x];
-            t += sm_l[i];
+            const float f = __builtin_amdgcn_exp2f(sm_m[i] - base);
+            v = fmaf(sm_o[i][threadIdx.x], f, v);
+            t = fmaf(sm_l[i], f, t);
         }
-        out[threadIdx.x] = top == -INFINITY && t == 0.f ? 0.f : v / t;
+        out[threadIdx.x] = all == -INFINITY && t == 0.f ? 0.f : v / t;
     }
 }
 
@@ -1188,28 +1212,43 @@ int launch_paged_select(int hd, const PagedView& kv, const float* q, const uint3
     return check_hip(hipGetLastError(), "paged_select launch");
 }
 
-// Workgroups that the steps are dealt out to, two a CU; a launch whose units hold no more than UNCUT keys has a workgroup for each and nothing to join.
-constexpr int LOG_WGS = 9, UNCUT = 512, MIN_STEPS = 8;
-size_t paged_attention_ws_bytes(const PagedView& kv, int hd, int n_head, size_t max_len) {
-    return max_len <= UNCUT ? 0 : ((size_t)2 << LOG_WGS) * (n_head / kv.n_kv) * (hd + 4) * sizeof(float);
+// Workgroups that the steps are dealt out to, two a CU.
+constexpr int LOG_WGS = 9, MIN_STEPS = 6;
+// Whether every unit has a workgroup of its own and nothing is joined: up to four steps for each of its waves; of more units than there are workgroups otherwise up to sixteen, which even
+// a single long sequence among short ones walks through in less time than the others' bytes take. us, own | dealt out, heads of 128: bf16 1 sequence of 400 keys and 8 KV heads 8.2 | 9.8, 32 of 400 12.6 | 18.5,
+// 64 of 500 28.6 | 33.2, 64 of 2000 97.9 | 103, but 8 of 2000 24.5 | 20.1.
+static bool own_workgroups(uint32_t type, const PagedView& kv, size_t keys) {
+    const size_t steps = (keys + (type == FHIP_F32 ? 15 : 31)) / (type == FHIP_F32 ? 16 : 32);
+    return steps <= 16 || ((size_t)kv.n_seq * kv.n_kv >= ((size_t)1 << LOG_WGS) && steps <= 64);
+}
+static size_t plan_floats(const PagedView& kv) { return ((size_t)kv.n_seq * kv.n_kv + 3) / 4 * 4; }
+size_t paged_attention_ws_bytes(uint32_t type, const PagedView& kv, int hd, int n_head, size_t max_len) {
+    return own_workgroups(type, kv, max_len) ? 0 : (plan_floats(kv) + ((size_t)2 << LOG_WGS) * (n_head / kv.n_kv) * (hd + 4)) * sizeof(float);
 }
 int launch_paged_attention(uint32_t type, int hd, const PagedView& kv, const float* q, const uint32_t* lens, uint32_t max_len, const uint32_t* selected, uint32_t n_select,
                            int n_head, uint32_t window, float softcap, float* ws, float* out, hipStream_t s) {
+    const size_t units = (size_t)kv.n_seq * kv.n_kv;
+    size_t keys = selected ? (size_t)n_select << kv.shift : max_len;
+    if (window > 0 && (size_t)window + 31 < keys) keys = (size_t)window + 31;      // a window begins and ends within steps
+    if ((size_t)kv.n_seq * n_head > 0x7FFFFFull) return set_error(FHIP_ERR_SHAPE, "paged attention: too many sequences and heads for one launch");
     Attend a;
-    a.kv = kv; a.q = q; a.lens = lens; a.selected = selected; a.out = out; a.part = ws;
+    a.kv = kv; a.q = q; a.lens = lens; a.selected = selected; a.out = out; a.plan = (uint32_t*)ws; a.part = ws + plan_floats(kv);
     a.max_len = max_len; a.n_select = n_select; a.window = window; a.n_head = n_head; a.softcap = softcap; a.scale = 1.0f / sqrtf((float)hd);
-    const size_t keys = selected ? (size_t)n_select << kv.shift : max_len;
-    a.log_wgs = keys <= UNCUT ? -1 : LOG_WGS;
+    a.log_wgs = own_workgroups(type, kv, keys) ? -1 : LOG_WGS;
     a.min_steps = MIN_STEPS;
-    const dim3 grid(a.log_wgs < 0 ? kv.n_seq * kv.n_kv : 1u << LOG_WGS);
+    const bool alone = a.log_wgs < 0 && units > 4 * (size_t)device_cus();      // more units than the chip has waves for by fours: a wave each
+    const dim3 grid(a.log_wgs < 0 ? (unsigned)units : 1u << LOG_WGS);
     return by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
-        auto go = [&](auto kernel, auto join) {
-            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a);
-            if (a.log_wgs >= 0) hipLaunchKernelGGL(join, dim3(kv.n_seq * (unsigned)n_head), dim3(256), 0, s, a);
+        auto go = [&](auto dims, auto sel) {
+            constexpr int HD = decltype(dims)::value;
+            constexpr bool SEL = decltype(sel)::value;
+            if (alone) hipLaunchKernelGGL((attention_kernel<TYPE, HD, SEL, 1>), grid, dim3(64), 0, s, a);
+            else hipLaunchKernelGGL((attention_kernel<TYPE, HD, SEL, 4>), grid, dim3(256), 0, s, a);
+            if (a.log_wgs >= 0) hipLaunchKernelGGL((join_kernel<TYPE, HD, SEL>), dim3(kv.n_seq * (unsigned)n_head), dim3(256), 0, s, a);
         };
-        if (hd == 128) selected ? go(attention_kernel<TYPE, 128, true, 4>, join_kernel<TYPE, 128, true>) : go(attention_kernel<TYPE, 128, false, 4>, join_kernel<TYPE, 128, false>);
-        else selected ? go(attention_kernel<TYPE, 64, true, 4>, join_kernel<TYPE, 64, true>) : go(attention_kernel<TYPE, 64, false, 4>, join_kernel<TYPE, 64, false>);
+        auto at = [&](auto sel) { hd == 128 ? go(std::integral_constant<int, 128>(), sel) : go(std::integral_constant<int, 64>(), sel); };
+        selected ? at(std::true_type()) : at(std::false_type());
         return check_hip(hipGetLastError(), "paged_attention launch");
     });
 }

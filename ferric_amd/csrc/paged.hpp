@@ -30,7 +30,7 @@ size_t paged_select_ws_bytes(const PagedView& kv, size_t max_len);
 int launch_paged_select(int hd, const PagedView& kv, const float* q, const uint32_t* lens, uint32_t max_len, const float* bounds, int n_head, uint32_t n_select,
                         uint32_t first, uint32_t last, void* ws, uint32_t* out, hipStream_t s);
 // selected: null, or [n_seq, n_kv, n_select] page indices of the sequences
-size_t paged_attention_ws_bytes(const PagedView& kv, int hd, int n_head, size_t max_len);
+size_t paged_attention_ws_bytes(uint32_t type, const PagedView& kv, int hd, int n_head, size_t max_len);
 int launch_paged_attention(uint32_t type, int hd, const PagedView& kv, const float* q, const uint32_t* lens, uint32_t max_len, const uint32_t* selected, uint32_t n_select,
                            int n_head, uint32_t window, float softcap, float* ws, float* out, hipStream_t s);
 

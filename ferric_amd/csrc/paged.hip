@@ -360,21 +360,30 @@ __global__ __launch_bounds__(256, 2) void score_kernel(PagedView kv, const float
 
 // The n_select largest keys of a list, equal ones by their place, as ascending places. One workgroup a list. The key that the last chosen one has is found by counting: the
 // interval that holds it is cut into 1024 by its width, and the one of these with it is the next interval.
-constexpr int SEL_T = 1024, SEL_BINS = 1024, SEL_HELD = 8;
+// T threads; HELD: they keep the keys in registers, up to HELD neighbouring ones each (0, for more than T * HELD: they read them again for each pass). With the keys read
+// again for every pass 2048 pages took 16.6 us, from registers of 1024 threads, the 256 first of which had all of them, 13.5.
+constexpr int SEL_BINS = 1024, SEL_HELD = 8;
+// A wave's inclusive sum.
+__device__ __forceinline__ uint32_t wave_upto(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);      // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);      // row_bcast 15 into rows 1 and 3, 31 into rows 2 and 3
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);
+    return v;
+}
 // Over the workgroup: each thread's sum of those in front of it, and of all. buf: a word for each wave.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* buf, int lane, int wave, uint32_t& all) {
-    uint32_t upto = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t t = __shfl_up(upto, o);
-        if (lane >= o) upto += t;
-    }
+template <int T>
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* buf, uint32_t& all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t upto = wave_upto(v);
     __syncthreads();
     if (lane == 63) buf[wave] = upto;
     __syncthreads();
     uint32_t before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < SEL_T / 64; w++) {
+    for (int w = 0; w < T / 64; w++) {
         const uint32_t c = buf[w];
         before += w < wave ? c : 0;
         total += c;
@@ -382,12 +391,12 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* buf, int la
     all = total;
     return before + upto - v;
 }
-// HELD: the keys stay in registers, SEL_HELD neighbouring ones a thread; otherwise (more than SEL_T * SEL_HELD) they are read again for each pass.
-template <bool HELD>
-__global__ __launch_bounds__(SEL_T) void select_kernel(PagedView kv, const uint32_t* __restrict__ lens, uint32_t max_len, uint32_t n_select, const uint64_t* __restrict__ keys,
-                                                       uint32_t key_stride, uint32_t kept, uint32_t* __restrict__ out) {
-    __shared__ uint32_t hist[SEL_BINS], buf[SEL_T / 64];
-    __shared__ uint64_t edge[2][SEL_T / 64];
+template <int T, int HELD>
+__global__ __launch_bounds__(T) void select_kernel(PagedView kv, const uint32_t* __restrict__ lens, uint32_t max_len, uint32_t n_select, const uint64_t* __restrict__ keys,
+                                                   uint32_t key_stride, uint32_t kept, uint32_t* __restrict__ out) {
+    constexpr int BPT = SEL_BINS / T;                 // bins a thread
+    __shared__ uint32_t hist[SEL_BINS], buf[T / 64];
+    __shared__ uint64_t edge[2][T / 64];
     __shared__ uint32_t found[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t list = blockIdx.x, seq = list / kv.n_kv;
@@ -395,21 +404,22 @@ __global__ __launch_bounds__(SEL_T) void select_kernel(PagedView kv, const uint3
     keys += (size_t)list * key_stride;
     out += (size_t)list * n_select;
     if (n <= n_select) {
-        for (uint32_t j = tid; j < n_select; j += SEL_T) out[j] = j < n ? j : NO_PAGE;
+        for (uint32_t j = tid; j < n_select; j += T) out[j] = j < n ? j : NO_PAGE;
         return;
     }
-    uint64_t held[SEL_HELD];
-    if (HELD)
+    const uint32_t per = (n + T - 1) / T, first = tid * per;      // HELD: this thread's keys are first .. first + per - 1
+    uint64_t held[HELD ? HELD : 1];
+    if constexpr (HELD > 0)
 #pragma unroll
-        for (int e = 0; e < SEL_HELD; e++) held[e] = tid * SEL_HELD + e < n ? keys[tid * SEL_HELD + e] : 0;
+        for (int e = 0; e < HELD; e++) held[e] = (uint32_t)e < per && first + e < n ? keys[first + e] : 0;
     // f(key, place) of this thread's keys, in their order where HELD
     auto each = [&](auto f) {
-        if constexpr (HELD) {
+        if constexpr (HELD > 0) {
 #pragma unroll
-            for (int e = 0; e < SEL_HELD; e++)
-                if (tid * SEL_HELD + e < n) f(held[e], (uint32_t)(tid * SEL_HELD + e));
+            for (int e = 0; e < HELD; e++)
+                if ((uint32_t)e < per && first + e < n) f(held[e], first + e);
         } else {
-            for (uint32_t j = tid; j < n; j += SEL_T) f(keys[j], j);
+            for (uint32_t j = tid; j < n; j += T) f(keys[j], j);
         }
     };
     uint64_t lo = ~0ull, hi = 0;
@@ -418,17 +428,20 @@ __global__ __launch_bounds__(SEL_T) void select_kernel(PagedView kv, const uint3
         lo = k < lo ? k : lo;
         hi = k > hi ? k : hi;
     });
+    lo = row16(lo, [](uint64_t a, uint64_t b) { return a < b ? a : b; });
+    hi = row16(hi, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
 #pragma unroll
-    for (int o = 32; o; o >>= 1) {
+    for (int o = 16; o < 64; o <<= 1) {
         const uint64_t a = __shfl_xor((unsigned long long)lo, o), b = __shfl_xor((unsigned long long)hi, o);
         lo = a < lo ? a : lo;
         hi = b > hi ? b : hi;
     }
     if (lane == 0) { edge[0][wave] = lo; edge[1][wave] = hi; }
-    hist[tid] = 0;
+#pragma unroll
+    for (int e = 0; e < BPT; e++) hist[tid + T * e] = 0;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < SEL_T / 64; w++) {
+    for (int w = 0; w < T / 64; w++) {
         lo = edge[0][w] < lo ? edge[0][w] : lo;
         hi = edge[1][w] > hi ? edge[1][w] : hi;
     }
@@ -439,14 +452,22 @@ __global__ __launch_bounds__(SEL_T) void select_kernel(PagedView kv, const uint3
             if (k >= lo && k <= hi) atomicAdd(&hist[(uint32_t)((k - lo) >> shift)], 1u);
         });
         __syncthreads();
-        const uint32_t mine = hist[SEL_BINS - 1 - tid];      // the highest bin first
-        uint32_t all;
-        const uint32_t above = block_scan(mine, buf, lane, wave, all);
-        if (above < want && above + mine >= want) {
-            found[0] = SEL_BINS - 1 - tid;
-            found[1] = want - above;
+        uint32_t mine[BPT], sum = 0, all;             // this thread's bins, the highest first
+#pragma unroll
+        for (int e = 0; e < BPT; e++) {
+            const int bin = SEL_BINS - 1 - (tid * BPT + e);
+            sum += mine[e] = hist[bin];
+            hist[bin] = 0;
         }
-        hist[SEL_BINS - 1 - tid] = 0;
+        uint32_t above = block_scan<T>(sum, buf, all);
+#pragma unroll
+        for (int e = 0; e < BPT; e++) {
+            if (above < want && above + mine[e] >= want) {
+                found[0] = SEL_BINS - 1 - (tid * BPT + e);
+                found[1] = want - above;
+            }
+            above += mine[e];
+        }
         __syncthreads();
         const uint64_t bin = found[0];
         if (bin < (hi - lo) >> shift) hi = lo + ((bin + 1) << shift) - 1;
@@ -457,27 +478,27 @@ __global__ __launch_bounds__(SEL_T) void select_kernel(PagedView kv, const uint3
     auto above = [&](uint64_t k) { return k == ~0ull || (want > 0 && k > lo); };
     auto equal = [&](uint64_t k) { return k == lo && k != ~0ull; };
     uint32_t all;
-    if constexpr (HELD) {
+    if constexpr (HELD > 0) {
         uint32_t same = 0, take = 0;
         each([&](uint64_t k, uint32_t) { same += equal(k); });
-        uint32_t rank = block_scan(same, buf, lane, wave, all);
+        uint32_t rank = block_scan<T>(same, buf, all);
         const uint32_t rank0 = rank;
         each([&](uint64_t k, uint32_t) { take += above(k) || (equal(k) && rank++ < want); });
-        uint32_t at = block_scan(take, buf, lane, wave, all);
+        uint32_t at = block_scan<T>(take, buf, all);
         rank = rank0;
         each([&](uint64_t k, uint32_t j) {
             if (above(k) || (equal(k) && rank++ < want)) out[at++] = j;
         });
     } else {
         uint32_t done = 0, ties = 0;
-        for (uint32_t j0 = 0; j0 < n; j0 += SEL_T) {
+        for (uint32_t j0 = 0; j0 < n; j0 += T) {
             const uint32_t j = j0 + tid;
             const uint64_t k = j < n ? keys[j] : 0;
             const bool same = j < n && equal(k);
-            const uint32_t rank = ties + block_scan(same, buf, lane, wave, all);
+            const uint32_t rank = ties + block_scan<T>(same, buf, all);
             ties += all;
             const bool take = j < n && (above(k) || (same && rank < want));
-            const uint32_t at = done + block_scan(take, buf, lane, wave, all);
+            const uint32_t at = done + block_scan<T>(take, buf, all);
             done += all;
             if (take) out[at] = j;
         }
@@ -1207,8 +1228,12 @@ int launch_paged_select(int hd, const PagedView& kv, const float* q, const uint3
         else hipLaunchKernelGGL((score_kernel<64>), grid, dim3(256), 0, s, kv, q, lens, max_len, bounds, n_head, first, last, (uint64_t*)ws, pages);
     }
     const dim3 lists(kv.n_seq * kv.n_kv);
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, lists, dim3(SEL_T), 0, s, kv, lens, max_len, n_select, (const uint64_t*)ws, pages, first + last, out); };
-    pages <= SEL_T * SEL_HELD ? go(select_kernel<true>) : go(select_kernel<false>);
+    auto go = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, lists, dim3(threads), 0, s, kv, lens, max_len, n_select, (const uint64_t*)ws, pages, first + last, out);
+    };
+    if (pages <= 256 * SEL_HELD) go(select_kernel<256, SEL_HELD>, 256);
+    else if (pages <= 1024 * SEL_HELD) go(select_kernel<1024, SEL_HELD>, 1024);
+    else go(select_kernel<1024, 0>, 1024);
     return check_hip(hipGetLastError(), "paged_select launch");
 }
 

@@ -397,7 +397,7 @@ __global__ __launch_bounds__(T) void select_kernel(PagedView kv, const uint32_t*
     constexpr int BPT = SEL_BINS / T;                 // bins a thread
     __shared__ uint32_t hist[SEL_BINS], buf[T / 64];
     __shared__ uint64_t edge[2][T / 64];
-    __shared__ uint32_t found[2];
+    __shared__ uint32_t found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const uint32_t list = blockIdx.x, seq = list / kv.n_kv;
     const uint32_t n = pages_of(kv, rows_of(kv, lens, seq, max_len));
@@ -445,8 +445,10 @@ __global__ __launch_bounds__(T) void select_kernel(PagedView kv, const uint32_t*
         lo = edge[0][w] < lo ? edge[0][w] : lo;
         hi = edge[1][w] > hi ? edge[1][w] : hi;
     }
-    uint32_t want = n_select - kept;                  // of the keys within [lo, hi], the largest `want` are chosen; here n > n_select >= kept, so it holds some
-    while (want > 0 && lo < hi) {                     // (hist is clear here)
+    // Chosen are the keys above hi and the largest `want` within [lo, hi]; here n > n_select >= kept, so that holds some. It is over when all that it holds are wanted, or are equal.
+    uint32_t want = n_select - kept;
+    if (want == 0) lo = hi = ~0ull;
+    while (lo < hi) {                                 // (hist is clear here)
         const int bits = 64 - __builtin_clzll(hi - lo), shift = bits > 10 ? bits - 10 : 0;      // (hi - lo) >> shift < 1024
         each([&](uint64_t k, uint32_t) {
             if (k >= lo && k <= hi) atomicAdd(&hist[(uint32_t)((k - lo) >> shift)], 1u);
@@ -465,6 +467,7 @@ __global__ __launch_bounds__(T) void select_kernel(PagedView kv, const uint32_t*
             if (above < want && above + mine[e] >= want) {
                 found[0] = SEL_BINS - 1 - (tid * BPT + e);
                 found[1] = want - above;
+                found[2] = mine[e];
             }
             above += mine[e];
         }
@@ -473,9 +476,13 @@ __global__ __launch_bounds__(T) void select_kernel(PagedView kv, const uint32_t*
         if (bin < (hi - lo) >> shift) hi = lo + ((bin + 1) << shift) - 1;
         lo += bin << shift;
         want = found[1];
+        if (want == found[2] && lo > 0) {             // all of them: those above lo - 1
+            hi = --lo;
+            want = 0;
+        }
     }
-    // places of the keys above it, and of the first `want` that equal it
-    auto above = [&](uint64_t k) { return k == ~0ull || (want > 0 && k > lo); };
+    // places of the keys above lo, and of the first `want` that equal it
+    auto above = [&](uint64_t k) { return k == ~0ull || k > lo; };
     auto equal = [&](uint64_t k) { return k == lo && k != ~0ull; };
     uint32_t all;
     if constexpr (HELD > 0) {
@@ -1139,13 +1146,29 @@ __global__ __launch_bounds__(256) void join_kernel(Attend a) {
     const int group = threadIdx.x / LANES, d = 4 * (threadIdx.x % LANES);
     f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY, sum = 0.f;
-    for (uint32_t w = w0 + group; w <= w1; w += GROUPS) {
-        const float* p = part(w);
-        const float m = p[g * HD + 2 * h], l = p[g * HD + 2 * h + 1];
-        const f32x4 v = *(const f32x4*)(p + h * HD + d);
-        const float now = fmaxf(top, m), base = now == -INFINITY ? 0.f : now, f0 = __builtin_amdgcn_exp2f(top - base), f1 = __builtin_amdgcn_exp2f(m - base);
-        o = o * f0 + v * f1;
-        sum = fmaf(l, f1, sum * f0);
+    for (uint32_t w = w0 + group; w <= w1; w += 4 * GROUPS) {      // four shares requested together
+        float m[4], l[4];
+        f32x4 v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t at = w + e * GROUPS;
+            const float* p = part(at <= w1 ? at : w);
+            m[e] = at <= w1 ? p[g * HD + 2 * h] : -INFINITY;
+            l[e] = p[g * HD + 2 * h + 1];
+            v[e] = *(const f32x4*)(p + h * HD + d);
+        }
+        float now = top;
+#pragma unroll
+        for (int e = 0; e < 4; e++) now = fmaxf(now, m[e]);
+        const float base = now == -INFINITY ? 0.f : now, f0 = __builtin_amdgcn_exp2f(top - base);
+        o *= f0;
+        sum *= f0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float f = w + e * GROUPS <= w1 ? __builtin_amdgcn_exp2f(m[e] - base) : 0.f;
+            o += w + e * GROUPS <= w1 ? v[e] * f : (f32x4){0.f, 0.f, 0.f, 0.f};
+            sum += w + e * GROUPS <= w1 ? l[e] * f : 0.f;
+        }
         top = now;
     }
     *(f32x4*)&sm_o[group][d] = o;

@@ -1700,7 +1700,7 @@ static int paged_view(const char* who, const fhip_paged* kv, fhip::PagedView& v)
         return set_error(FHIP_ERR_SHAPE, "%s: page_rows must be a power of two from 16 to 4096, got %u", who, kv->page_rows);
     if (kv->n_kv < 1 || kv->n_kv > 4096) return set_error(FHIP_ERR_SHAPE, "%s: n_kv must be 1..=4096, got %zu", who, kv->n_kv);
     if (kv->n_seq > 65535) return set_error(FHIP_ERR_SHAPE, "%s: more than 65535 sequences", who);
-    if (kv->n_pages > 0xFFFFFFFEull) return set_error(FHIP_ERR_SHAPE, "%s: more than 2^32 - 2 pages", who);
+    if (kv->n_pages < 1 || kv->n_pages > 0xFFFFFFFEull) return set_error(FHIP_ERR_SHAPE, "%s: n_pages must be 1..=2^32 - 2, got %zu", who, kv->n_pages);
     if (kv->pages_per_seq > 0xFFFFFFFFull / kv->page_rows) return set_error(FHIP_ERR_SHAPE, "%s: a sequence's rows reach 2^32", who);
     if (kv->table_stride < kv->pages_per_seq) return set_error(FHIP_ERR_SHAPE, "%s: table_stride %zu is less than pages_per_seq %zu", who, kv->table_stride, kv->pages_per_seq);
     if (!kv->d_k || !kv->d_v || !aligned16(kv->d_k) || !aligned16(kv->d_v)) return set_error(FHIP_ERR_ARG, "%s: the pools must be 16-byte aligned device memory", who);

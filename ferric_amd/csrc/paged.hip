@@ -307,54 +307,51 @@ __device__ __forceinline__ uint64_t order_key(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     return b >> 63 ? ~b : b | 1ull << 63;
 }
-// On v_mfma_f64_16x16x4_f64: 16 pages by the head's queries, max(q, 0) and min(q, 0) in f64 in registers, a lane's bounds four neighbouring dims of a page at a time. Bound by the
-// bounds' bytes: the instructions of 16 pages take 4096 cycles, 9.8 TB/s of bounds on the chip. A wave a page, with a sum over its lanes for each query, took 75 us of 24 sequences of 4 KV heads of 8, 52 MB.
+// On v_mfma_f64_16x16x4_f64: 16 pages by the head's queries, max(q, 0) and min(q, 0) in f64 in LDS as the instructions take them, a lane's bounds four neighbouring dims of a page at a
+// time. Bound by the bounds' bytes: the instructions of 16 pages take 4096 cycles, 9.8 TB/s of bounds on the chip. us for 24 sequences' 52 MB of bounds: a wave a page, with a sum over its lanes for each
+// query, 75; with the queries in every wave's registers, two waves a SIMD, 24.5; so 20.
 template <int HD>
-__global__ __launch_bounds__(256, 2) void score_kernel(PagedView kv, const float* __restrict__ q, const uint32_t* __restrict__ lens, uint32_t max_len, const float* __restrict__ bounds,
-                                                       int n_head, uint32_t first, uint32_t last, uint64_t* __restrict__ keys, uint32_t key_stride) {
+__global__ __launch_bounds__(256) void score_kernel(PagedView kv, const float* __restrict__ q, const uint32_t* __restrict__ lens, uint32_t max_len, const float* __restrict__ bounds,
+                                                    int n_head, uint32_t first, uint32_t last, uint64_t* __restrict__ keys, uint32_t key_stride) {
     constexpr int NI = HD / 16;
+    __shared__ double up[4 * NI][64], down[4 * NI][64];
     const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4, g = n_head / kv.n_kv, head = blockIdx.y;
     const uint32_t seq = blockIdx.z, pages = pages_of(kv, rows_of(kv, lens, seq, max_len)), groups = (pages + 15) / 16;
+    if (blockIdx.x * 4 >= groups) return;
     uint32_t j = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (j >= groups) return;
     const uint32_t* table = kv.table + seq * kv.table_stride;
     keys += ((size_t)seq * kv.n_kv + head) * key_stride;
-    double up[NI][4], down[NI][4];
+    uint32_t mine = j < groups && 16 * j + n < pages ? table[16 * j + n] : NO_PAGE;
     const float* qh = q + ((size_t)seq * n_head + head * g + (n < g ? n : 0)) * HD + 4 * kg;
 #pragma unroll
-    for (int i = 0; i < NI; i++) {
+    for (int i = threadIdx.x >> 6; i < NI; i += 4) {
         const f32x4 x = *(const f32x4*)(qh + 16 * i);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            up[i][e] = x[e] > 0.f || x[e] != x[e] ? (double)x[e] : 0.0;
-            down[i][e] = x[e] < 0.f ? (double)x[e] : 0.0;
+            up[4 * i + e][lane] = x[e] < 0.f ? 0.0 : (double)x[e];      // (no number stays one)
+            down[4 * i + e][lane] = x[e] < 0.f ? (double)x[e] : 0.0;
         }
     }
-    for (; j < groups; j += gridDim.x * 4) {
-        const uint32_t mine = 16 * j + n < pages ? table[16 * j + n] : NO_PAGE;
-        const float* b = bounds + ((size_t)(mine < kv.n_pages ? mine : 0) * kv.n_kv + head) * 2 * HD + 4 * kg;
-        f32x4 lo[NI], hi[NI];
+    __syncthreads();
+    if (j >= groups) return;
+    const float* b = bounds + ((size_t)(mine < kv.n_pages ? mine : 0) * kv.n_kv + head) * 2 * HD + 4 * kg;
+    f64x4 s = (f64x4){0, 0, 0, 0}, s2 = s;
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            lo[i] = *(const f32x4*)(b + 16 * i);
-            hi[i] = *(const f32x4*)(b + HD + 16 * i);
+    for (int i = 0; i < NI; i++) {
+        const f32x4 lo = *(const f32x4*)(b + 16 * i), hi = *(const f32x4*)(b + HD + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            s = __builtin_amdgcn_mfma_f64_16x16x4f64((double)hi[e], up[4 * i + e][lane], s, 0, 0, 0);
+            s2 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)lo[e], down[4 * i + e][lane], s2, 0, 0, 0);
         }
-        f64x4 s = (f64x4){0, 0, 0, 0}, s2 = s;
+    }
 #pragma unroll
-        for (int i = 0; i < NI; i++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                s = __builtin_amdgcn_mfma_f64_16x16x4f64((double)hi[i][e], up[i][e], s, 0, 0, 0);
-                s2 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)lo[i][e], down[i][e], s2, 0, 0, 0);
-            }
-#pragma unroll
-        for (int r = 0; r < 4; r++) {                 // page 16 j + 4 r + kg, query n
-            const uint32_t page = 16 * j + 4 * r + kg;
-            const bool there = __shfl(mine, 4 * r + kg) < kv.n_pages;
-            uint64_t key = n < g && there ? order_key(s[r] + s2[r]) : order_key(-INFINITY);
-            key = row16(key, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-            if (n == 0 && page < pages) keys[page] = page < first || page + last >= pages ? ~0ull : key;
-        }
+    for (int r = 0; r < 4; r++) {                     // page 16 j + 4 r + kg, query n
+        const uint32_t page = 16 * j + 4 * r + kg;
+        const bool there = __shfl(mine, 4 * r + kg) < kv.n_pages;
+        uint64_t key = n < g && there ? order_key(s[r] + s2[r]) : order_key(-INFINITY);
+        key = row16(key, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+        if (n == 0 && page < pages) keys[page] = page < first || page + last >= pages ? ~0ull : key;
     }
 }
 
@@ -612,7 +609,7 @@ template <int TYPE, bool SEL>
 __device__ __forceinline__ Span span_of(const PagedView& kv, const uint32_t* __restrict__ lens, uint32_t seq, uint32_t max_len, uint32_t window, uint32_t n_select) {
     constexpr int KEYS = Path<TYPE>::KEYS;
     Span s;
-    s.len = kv.n_pages ? rows_of(kv, lens, seq, max_len) : 0;
+    s.len = rows_of(kv, lens, seq, max_len);
     s.lo = window && window < s.len ? s.len - window : 0;
     if constexpr (SEL) {
         const uint32_t pages = pages_of(kv, s.len), listed = pages < n_select ? pages : n_select;

@@ -446,7 +446,7 @@ int fhip_qkv_post_attention_kvq(int fmt, const float* d_qkv, const float* d_bias
  * values; position p of sequence i is row table[i * table_stride + p / page_rows] * page_rows + p % page_rows of the pools. Several sequences may name one page
  * (a common prefix). A table entry that is no page of the pool (n_pages and more) has no rows: what would be stored there is dropped, what would be read is left out.
  * Checked by every call below: type one of FHIP_F32, FHIP_F16, FHIP_BF16, FHIP_Q8_0 (FHIP_ERR_UNSUPPORTED_TYPE); head_dim 64 or 128; page_rows a power of two from 16 to 4096;
- * n_kv from 1 to 4096; n_seq up to 65535; up to 2^32 - 2 pages, a sequence's rows below 2^32; table_stride at least pages_per_seq (FHIP_ERR_SHAPE); pools 16-byte aligned, scales not NULL for Q8_0 (FHIP_ERR_ARG). */
+ * n_kv from 1 to 4096; n_seq up to 65535; 1 to 2^32 - 2 pages, a sequence's rows below 2^32; table_stride at least pages_per_seq (FHIP_ERR_SHAPE); pools 16-byte aligned, scales not NULL for Q8_0 (FHIP_ERR_ARG). */
 typedef struct fhip_paged {
     uint32_t type;            /* what the pools hold */
     uint32_t page_rows;

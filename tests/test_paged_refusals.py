@@ -29,7 +29,7 @@ def calls(kv, n_head=4):
     (dict(type=12), TYPE, "ggml type 12"), (dict(type=2), TYPE, "F32, F16, BF16 or Q8_0"),
     (dict(head_dim=96), SHAPE, "head_dim must be 64 or 128"), (dict(head_dim=0), SHAPE, "head_dim"),
     (dict(page_rows=8), SHAPE, "page_rows"), (dict(page_rows=48), SHAPE, "power of two"), (dict(page_rows=8192), SHAPE, "page_rows"), (dict(page_rows=0), SHAPE, "page_rows"),
-    (dict(n_kv=0), SHAPE, "n_kv"), (dict(n_kv=4097), SHAPE, "n_kv"), (dict(n_seq=65536), SHAPE, "65535"), (dict(n_pages=2 ** 32 - 1), SHAPE, "pages"),
+    (dict(n_kv=0), SHAPE, "n_kv"), (dict(n_kv=4097), SHAPE, "n_kv"), (dict(n_seq=65536), SHAPE, "65535"), (dict(n_pages=2 ** 32 - 1), SHAPE, "pages"), (dict(n_pages=0), SHAPE, "pages"),
     (dict(pages_per_seq=2 ** 28, table_stride=2 ** 28), SHAPE, "2^32"), (dict(table_stride=3), SHAPE, "table_stride"),
     (dict(d_k=None), ARG, "pools"), (dict(d_v=P + 8), ARG, "16-byte"), (dict(type=8), ARG, "scales"), (dict(type=8, d_k_scales=P, d_v_scales=P + 2), ARG, "scales"),
     (dict(d_table=None), ARG, "table")])

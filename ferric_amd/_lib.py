@@ -232,6 +232,8 @@ try:
     _host.setup(_host_first_use, check)
     DeviceBuffer, matmul_q = _host.DeviceBuffer, _host.matmul_q
     moe_topk, swiglu_id, id_wsum = _host.moe_topk, _host.swiglu_id, _host.id_wsum
+    paged_append, paged_attention, paged_attention_selected = _host.paged_append, _host.paged_attention, _host.paged_attention_selected
+    paged_key_bounds, paged_select, paged_rows = _host.paged_key_bounds, _host.paged_select, _host.paged_rows
 except (ImportError, AttributeError) as _e:      # not built, or built from older source
     _why = str(_e)
 

@@ -5,7 +5,8 @@
 // 4.4 us. A C type over the library's fhip_malloc / fhip_free does the same in a few hundred nanoseconds. A launch itself costs
 // the host 3 us on this runtime (0.9 us without arguments: the argument block is written to device memory and read back), which is
 // most of what is left of such a call, so matmul_q does all of its conversions here instead of in ctypes, and the three calls of routed experts do: through ctypes
-// they took the host 21.5 us where their kernels take 11 - 14, now 16 (1024 x 2048, 2 of 128 experts, one token 22.0 -> 15.8).
+// they took the host 21.5 us where their kernels take 11 - 14, now 16 (1024 x 2048, 2 of 128 experts, one token 22.0 -> 15.8). So do the paged cache's calls, whose
+// launches for a few sequences are as short.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <dlfcn.h>
@@ -20,8 +21,15 @@ int (*p_matmul_q)(const void*, const void*, size_t, void*, void*) = nullptr;
 int (*p_moe_topk)(const void*, const void*, size_t, size_t, size_t, int, float, int, void*, void*) = nullptr;
 int (*p_swiglu_id)(const void*, const void*, size_t, const void*, size_t, size_t, void*, void*) = nullptr;
 int (*p_id_wsum)(const void*, const void*, size_t, const void*, size_t, size_t, void*, void*, void*) = nullptr;
+int (*p_paged_append)(const void*, const void*, const void*, const void*, const void*, const void*, const void*, const void*, size_t, size_t, size_t, int, float, float, void*, void*) = nullptr;
+int (*p_paged_attention)(const void*, const void*, const void*, size_t, size_t, size_t, float, void*, void*, void*) = nullptr;
+int (*p_paged_selected)(const void*, const void*, const void*, const void*, size_t, size_t, float, void*, void*, void*) = nullptr;
+int (*p_paged_bounds)(const void*, const void*, const void*, size_t, void*, void*) = nullptr;
+int (*p_paged_select)(const void*, const void*, const void*, size_t, const void*, size_t, size_t, size_t, size_t, void*, void*, void*) = nullptr;
+int (*p_paged_rows)(const void*, size_t, size_t, size_t, void*, void*, void*) = nullptr;
 PyTypeObject* g_buffer_type = nullptr;
 PyObject* g_value = nullptr;         // "value"
+PyObject* g_ptr = nullptr;           // "ptr"
 PyObject* g_c_void_p = nullptr;      // ctypes.c_void_p
 PyObject* g_first_use = nullptr;     // called before the first allocation: initialises the device, calls bind()
 PyObject* g_check = nullptr;         // raises for a return code
@@ -260,6 +268,99 @@ PyObject* id_wsum(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return result(bytes, scratch, [&](void* y, void* ws) { return p_id_wsum(w, x, t, sel, d[0], d[1], y, ws, stream); });
 }
 
+// what a DeviceBuffer, another object with a `ptr`, an address or None stands for
+bool memory(PyObject* o, void** out) {
+    if (is_buffer(o)) { *out = ((Buffer*)o)->mem; return true; }
+    if (o == Py_None || PyLong_Check(o)) return address(o, out);
+    PyObject* p = PyObject_GetAttr(o, g_ptr);
+    if (!p) return false;
+    const bool ok = address(p, out);
+    Py_DECREF(p);
+    return ok;
+}
+bool memories(PyObject* const* a, int n, void** out) {
+    for (int i = 0; i < n; i++)
+        if (!memory(a[i], out + i)) return false;
+    return true;
+}
+PyObject* enqueued(int rc) {
+    if (rc) { raise_rc(rc); return nullptr; }
+    Py_RETURN_NONE;
+}
+// The paged cache's entry points: the description's address, memory (a DeviceBuffer, another object with a `ptr`, an address or None) and numbers in the library's order, the stream
+// as an address or None.
+PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 16) { PyErr_SetString(PyExc_TypeError, "paged_append: 16 arguments"); return nullptr; }
+    void *kv, *m[7], *q, *stream;
+    size_t d[3];
+    const int interleaved = PyObject_IsTrue(a[11]);
+    const float eps = (float)PyFloat_AsDouble(a[12]), base = (float)PyFloat_AsDouble(a[13]);
+    if (PyErr_Occurred() || ready() || !address(a[0], &kv) || !memories(a + 1, 7, m) || !sizes(a + 8, 3, d) || !memory(a[14], &q) || !address(a[15], &stream)) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_paged_append(kv, m[0], m[1], m[2], m[3], m[4], m[5], m[6], d[0], d[1], d[2], interleaved, eps, base, q, stream);
+    Py_END_ALLOW_THREADS
+    return enqueued(rc);
+}
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 10) { PyErr_SetString(PyExc_TypeError, "paged_attention: 10 arguments"); return nullptr; }
+    void *kv, *m[2], *o[2], *stream;
+    size_t d[3];
+    const float cap = (float)PyFloat_AsDouble(a[6]);
+    if (PyErr_Occurred() || ready() || !address(a[0], &kv) || !memories(a + 1, 2, m) || !sizes(a + 3, 3, d) || !memories(a + 7, 2, o) || !address(a[9], &stream)) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_paged_attention(kv, m[0], m[1], d[0], d[1], d[2], cap, o[0], o[1], stream);
+    Py_END_ALLOW_THREADS
+    return enqueued(rc);
+}
+PyObject* paged_attention_selected(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 10) { PyErr_SetString(PyExc_TypeError, "paged_attention_selected: 10 arguments"); return nullptr; }
+    void *kv, *m[3], *o[2], *stream;
+    size_t d[2];
+    const float cap = (float)PyFloat_AsDouble(a[6]);
+    if (PyErr_Occurred() || ready() || !address(a[0], &kv) || !memories(a + 1, 3, m) || !sizes(a + 4, 2, d) || !memories(a + 7, 2, o) || !address(a[9], &stream)) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_paged_selected(kv, m[0], m[1], m[2], d[0], d[1], cap, o[0], o[1], stream);
+    Py_END_ALLOW_THREADS
+    return enqueued(rc);
+}
+PyObject* paged_key_bounds(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 6) { PyErr_SetString(PyExc_TypeError, "paged_key_bounds: 6 arguments"); return nullptr; }
+    void *kv, *m[2], *b, *stream;
+    size_t most;
+    if (ready() || !address(a[0], &kv) || !memories(a + 1, 2, m) || !sizes(a + 3, 1, &most) || !memory(a[4], &b) || !address(a[5], &stream)) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_paged_bounds(kv, m[0], m[1], most, b, stream);
+    Py_END_ALLOW_THREADS
+    return enqueued(rc);
+}
+PyObject* paged_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 12) { PyErr_SetString(PyExc_TypeError, "paged_select: 12 arguments"); return nullptr; }
+    void *kv, *m[2], *b, *o[2], *stream;
+    size_t most, d[4];
+    if (ready() || !address(a[0], &kv) || !memories(a + 1, 2, m) || !sizes(a + 3, 1, &most) || !memory(a[4], &b) || !sizes(a + 5, 4, d) || !memories(a + 9, 2, o) || !address(a[11], &stream))
+        return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_paged_select(kv, m[0], m[1], most, b, d[0], d[1], d[2], d[3], o[0], o[1], stream);
+    Py_END_ALLOW_THREADS
+    return enqueued(rc);
+}
+PyObject* paged_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 7) { PyErr_SetString(PyExc_TypeError, "paged_rows: 7 arguments"); return nullptr; }
+    void *kv, *o[2], *stream;
+    size_t d[3];
+    if (ready() || !address(a[0], &kv) || !sizes(a + 1, 3, d) || !memories(a + 4, 2, o) || !address(a[6], &stream)) return nullptr;
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = p_paged_rows(kv, d[0], d[1], d[2], o[0], o[1], stream);
+    Py_END_ALLOW_THREADS
+    return enqueued(rc);
+}
+
 PyObject* setup(PyObject*, PyObject* args) {
     PyObject *first_use, *check;
     if (!PyArg_ParseTuple(args, "OO", &first_use, &check)) return nullptr;
@@ -280,8 +381,15 @@ PyObject* bind(PyObject*, PyObject* args) {
     p_moe_topk = (decltype(p_moe_topk))dlsym(lib, "fhip_moe_topk");
     p_swiglu_id = (decltype(p_swiglu_id))dlsym(lib, "fhip_matmul_q_swiglu_id");
     p_id_wsum = (decltype(p_id_wsum))dlsym(lib, "fhip_matmul_q_id_wsum");
+    p_paged_append = (decltype(p_paged_append))dlsym(lib, "fhip_paged_append");
+    p_paged_attention = (decltype(p_paged_attention))dlsym(lib, "fhip_paged_attention");
+    p_paged_selected = (decltype(p_paged_selected))dlsym(lib, "fhip_paged_attention_selected");
+    p_paged_bounds = (decltype(p_paged_bounds))dlsym(lib, "fhip_paged_key_bounds");
+    p_paged_select = (decltype(p_paged_select))dlsym(lib, "fhip_paged_select");
+    p_paged_rows = (decltype(p_paged_rows))dlsym(lib, "fhip_paged_rows");
     p_malloc = (int (*)(void**, size_t))dlsym(lib, "fhip_malloc");
-    if (!p_malloc || !p_free || !p_matmul_q || !p_moe_topk || !p_swiglu_id || !p_id_wsum) { p_malloc = nullptr; PyErr_Format(PyExc_ImportError, "%s does not export what it should", path); return nullptr; }
+    if (!p_malloc || !p_free || !p_matmul_q || !p_moe_topk || !p_swiglu_id || !p_id_wsum || !p_paged_append || !p_paged_attention || !p_paged_selected || !p_paged_bounds || !p_paged_select ||
+        !p_paged_rows) { p_malloc = nullptr; PyErr_Format(PyExc_ImportError, "%s does not export what it should", path); return nullptr; }
     Py_RETURN_NONE;
 }
 
@@ -290,6 +398,12 @@ PyMethodDef methods[] = {{"setup", setup, METH_VARARGS, "setup(first_use, check)
                          {"moe_topk", (PyCFunction)(void*)moe_topk, METH_FASTCALL, "moe_topk(logits, bias, tokens, experts, k, sigmoid, scale, norm, stream)"},
                          {"swiglu_id", (PyCFunction)(void*)swiglu_id, METH_FASTCALL, "swiglu_id(x, handle, tokens, selection, k, outputs, stream)"},
                          {"id_wsum", (PyCFunction)(void*)id_wsum, METH_FASTCALL, "id_wsum(x, handle, tokens, selection, k, outputs, stream)"},
+                         {"paged_append", (PyCFunction)(void*)paged_append, METH_FASTCALL, "fhip_paged_append"},
+                         {"paged_attention", (PyCFunction)(void*)paged_attention, METH_FASTCALL, "fhip_paged_attention"},
+                         {"paged_attention_selected", (PyCFunction)(void*)paged_attention_selected, METH_FASTCALL, "fhip_paged_attention_selected"},
+                         {"paged_key_bounds", (PyCFunction)(void*)paged_key_bounds, METH_FASTCALL, "fhip_paged_key_bounds"},
+                         {"paged_select", (PyCFunction)(void*)paged_select, METH_FASTCALL, "fhip_paged_select"},
+                         {"paged_rows", (PyCFunction)(void*)paged_rows, METH_FASTCALL, "fhip_paged_rows"},
                          {"bind", bind, METH_VARARGS, "bind(library path)"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Device memory objects of ferric_amd.", -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -301,7 +415,7 @@ PyMODINIT_FUNC PyInit__host(void) {
     if (!ctypes) return nullptr;
     g_c_void_p = PyObject_GetAttrString(ctypes, "c_void_p");
     Py_DECREF(ctypes);
-    if (!g_c_void_p || !(g_value = PyUnicode_InternFromString("value"))) return nullptr;
+    if (!g_c_void_p || !(g_value = PyUnicode_InternFromString("value")) || !(g_ptr = PyUnicode_InternFromString("ptr"))) return nullptr;
     PyObject* m = PyModule_Create(&module);
     if (!m) return nullptr;
     PyObject* type = PyType_FromSpec(&buffer_spec);

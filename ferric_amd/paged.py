@@ -10,15 +10,19 @@ import ctypes as C
 import numpy as np
 
 from . import _lib
-from .qmatrix import BF16, F16, F32, Q8_0, DeviceBuffer, Tensor, _arrived, _stream_handle, _upload
+from .qmatrix import BF16, F16, F32, Q8_0, DeviceBuffer, Tensor, _arrived, _upload
 
 ALL = (F32, F16, BF16, Q8_0)
 NO_PAGE = 0xFFFFFFFF
 _VALUE_BYTES = {F32: 4, F16: 2, BF16: 2, Q8_0: 1}
 
 
-def _ptr(t):
-    return None if t is None else t.buf.ptr
+def _buf(t):
+    return None if t is None else t.buf
+
+
+def _at(stream):
+    return None if stream is None else stream.handle
 
 
 class PagedKvCache:
@@ -48,8 +52,8 @@ class PagedKvCache:
         self.k, self.v, self.k_scales, self.v_scales, self.table, self.n_seq, self.pages_per_seq = k, v, k_scales, v_scales, table, n_seq, pages_per_seq
         at = lambda b: None if b is None else getattr(b.ptr, "value", b.ptr)      # noqa: E731
         self._desc = _lib.Paged(ty, page_rows, n_pages, n_kv, head_dim, at(k), at(v), at(k_scales), at(v_scales), at(table), n_seq, pages_per_seq, pages_per_seq)
-        self._ref = C.byref(self._desc)
-        self._ws = {}
+        self._ref, self._addr = C.byref(self._desc), C.addressof(self._desc)
+        self._ws, self._needs, self._rows = {}, {}, n_kv * head_dim
 
     def set_table(self, pages, stream=None):
         """The whole table from the host, [n_seq, pages_per_seq]; NO_PAGE (or any number past the pool) where a sequence has none."""
@@ -59,30 +63,46 @@ class PagedKvCache:
             _upload(self.table, a, stream)
             _arrived(a, stream)
 
-    def _workspace(self, need, ws, stream):
-        """The caller's, or one kept for the stream. What was outgrown stays: a graph captured on the stream may name it. Graphs that may run at the same time need
-        workspaces of their own."""
-        if ws is not None or need == 0:
-            return None if ws is None else ws.ptr
+    def _workspace(self, n_heads, keys, ws, stream):
+        """The caller's workspace, or one kept for the stream, for attention over `keys` keys a sequence (n_heads 0: for select). What was outgrown stays: a graph captured on
+        the stream may name it. Graphs that may run at the same time need workspaces of their own."""
+        if ws is not None:
+            return ws
+        at = n_heads, keys.bit_length()               # sized for the next power of two: asked for once
+        need = self._needs.get(at)
+        if need is None:
+            lib = _lib.load()
+            need = lib.fhip_paged_attention_ws_bytes(self._ref, n_heads, 1 << at[1]) if n_heads else lib.fhip_paged_select_ws_bytes(self._ref, 1 << at[1])
+            self._needs[at] = need
+        if need == 0:
+            return None
         kept = self._ws.setdefault(None if stream is None else stream.handle.value, [])
         if not kept or kept[-1].nbytes < need:
             kept.append(DeviceBuffer(1 << (need - 1).bit_length()))
-        return kept[-1].ptr
+        return kept[-1]
+
+    def reserve(self, n_heads, max_len, n_select=0, stream=None):
+        """Makes the workspace that attention (and, with n_select pages, select and attention_selected) of up to max_len keys takes on this stream, which a capture cannot."""
+        self._workspace(n_heads, max_len, None, stream)
+        if n_select:
+            self._workspace(0, max_len, None, stream)
+            self._workspace(n_heads, n_select * self.page_rows, None, stream)
 
     def append(self, qkv, seqs, positions, n_heads, base, n_rot=None, interleaved=False, eps=1e-6, bias=None, q_norm=None, k_norm=None, freq_scale=None, out=None, stream=None):
         """Post-processes the fused rows qkv [t, (n_heads + 2 n_kv) * head_dim] of t new tokens (bias, head norm, rotation), stores their keys and values, returns their
         queries [t, n_heads * head_dim]. seqs, positions: device u32 Tensors [t]; seqs None: token i is of sequence i."""
         t, width = qkv.shape
-        assert width == (n_heads + 2 * self.n_kv) * self.head_dim, f"append: rows of {width} values are not {n_heads} + 2 * {self.n_kv} heads of {self.head_dim}"
-        assert positions.numel() == t and (seqs is None or seqs.numel() == t), "append: one position and one sequence a row"
-        assert (bias is None or bias.numel() == width) and all(w is None or w.numel() == self.head_dim for w in (q_norm, k_norm)), "append: bias or norm of another size"
-        n_rot = self.head_dim if n_rot is None else n_rot
+        hd = self.head_dim
+        assert width == n_heads * hd + 2 * self._rows, f"append: rows of {width} values are not {n_heads} + 2 * {self.n_kv} heads of {hd}"
+        assert positions.numel() == t and (t <= self.n_seq if seqs is None else seqs.numel() == t), "append: one position and one sequence a row"
+        assert (bias is None or bias.numel() == width) and (q_norm is None or q_norm.numel() == hd) and (k_norm is None or k_norm.numel() == hd), "append: bias or norm of another size"
+        if n_rot is None:
+            n_rot = hd
         assert freq_scale is None or 2 * freq_scale.numel() >= n_rot, "append: a frequency scale for every pair"
-        assert seqs is not None or t <= self.n_seq, "append: more rows than sequences"
-        q = Tensor.empty((t, n_heads * self.head_dim)) if out is None else out
-        assert q.shape == (t, n_heads * self.head_dim), "append: out has another shape"
-        _lib.check(_lib.load().fhip_paged_append(self._ref, qkv.buf.ptr, _ptr(bias), _ptr(q_norm), _ptr(k_norm), _ptr(seqs), positions.buf.ptr, _ptr(freq_scale), t, n_heads, n_rot,
-                                                 int(interleaved), eps, base, q.buf.ptr, _stream_handle(stream)))
+        q = Tensor.empty((t, n_heads * hd)) if out is None else out
+        assert q.shape == (t, n_heads * hd), "append: out has another shape"
+        _lib.paged_append(self._addr, qkv.buf, _buf(bias), _buf(q_norm), _buf(k_norm), _buf(seqs), positions.buf, _buf(freq_scale), t, n_heads, n_rot, interleaved, eps, base, q.buf,
+                          _at(stream))
         return q
 
     def _query(self, q, lens, n_heads, out):
@@ -97,10 +117,7 @@ class PagedKvCache:
         """One new token of every sequence, q [n_seq, n_heads * head_dim], over the first lens[i] rows (device u32 Tensor, the new token's own among them; at most
         max_len) or the newest `window` of them."""
         out = self._query(q, lens, n_heads, out)
-        lib = _lib.load()
-        need = lib.fhip_paged_attention_ws_bytes(self._ref, n_heads, max_len)
-        _lib.check(lib.fhip_paged_attention(self._ref, q.buf.ptr, lens.buf.ptr, max_len, n_heads, window, softcap, self._workspace(need, ws, stream), out.buf.ptr,
-                                            _stream_handle(stream)))
+        _lib.paged_attention(self._addr, q.buf, lens.buf, max_len, n_heads, window, softcap, self._workspace(n_heads, max_len, ws, stream), out.buf, _at(stream))
         return out
 
     def empty_bounds(self):
@@ -111,7 +128,7 @@ class PagedKvCache:
         """Takes the keys of each sequence's last `fresh` rows (device u32 Tensor; None: max_new) into their pages' bounds, in place."""
         assert lens.numel() == self.n_seq and (fresh is None or fresh.numel() == self.n_seq), "one length a sequence"
         assert bounds.numel() == self.n_pages * self.n_kv * 2 * self.head_dim, "key_bounds: bounds of another size"
-        _lib.check(_lib.load().fhip_paged_key_bounds(self._ref, lens.buf.ptr, _ptr(fresh), max_new, bounds.buf.ptr, _stream_handle(stream)))
+        _lib.paged_key_bounds(self._addr, lens.buf, _buf(fresh), max_new, bounds.buf, _at(stream))
         return bounds
 
     def select(self, q, lens, max_len, bounds, n_heads, n_select, first=1, last=1, out=None, ws=None, stream=None):
@@ -121,10 +138,8 @@ class PagedKvCache:
         shape = (self.n_seq, self.n_kv, n_select)
         out = Tensor.empty(shape, np.uint32) if out is None else out
         assert out.shape == shape, "select: out has another shape"
-        lib = _lib.load()
-        need = lib.fhip_paged_select_ws_bytes(self._ref, max_len)
-        _lib.check(lib.fhip_paged_select(self._ref, q.buf.ptr, lens.buf.ptr, max_len, bounds.buf.ptr, n_heads, n_select, first, last, self._workspace(need, ws, stream), out.buf.ptr,
-                                         _stream_handle(stream)))
+        _lib.paged_select(self._addr, q.buf, lens.buf, max_len, bounds.buf, n_heads, n_select, first, last, self._workspace(0, max_len, ws, stream), out.buf,
+                          _at(stream))
         return out
 
     def attention_selected(self, q, lens, selected, n_heads, softcap=0.0, out=None, ws=None, stream=None):
@@ -132,16 +147,14 @@ class PagedKvCache:
         out = self._query(q, lens, n_heads, out)
         assert selected.shape[:2] == (self.n_seq, self.n_kv) and len(selected.shape) == 3, "selected is [n_seq, n_kv, n]"
         n = selected.shape[2]
-        lib = _lib.load()
-        need = lib.fhip_paged_attention_ws_bytes(self._ref, n_heads, n * self.page_rows)
-        _lib.check(lib.fhip_paged_attention_selected(self._ref, q.buf.ptr, lens.buf.ptr, selected.buf.ptr, n, n_heads, softcap, self._workspace(need, ws, stream), out.buf.ptr,
-                                                     _stream_handle(stream)))
+        ws = self._workspace(n_heads, n * self.page_rows, ws, stream)
+        _lib.paged_attention_selected(self._addr, q.buf, lens.buf, selected.buf, n, n_heads, softcap, ws, out.buf, _at(stream))
         return out
 
     def rows(self, seq, row0, rows, out=None, stream=None):
         """Rows row0 .. row0 + rows of sequence seq as f32: (k, v), [rows, n_kv * head_dim] each."""
-        shape = (rows, self.n_kv * self.head_dim)
+        shape = (rows, self._rows)
         k, v = (Tensor.empty(shape), Tensor.empty(shape)) if out is None else out
         assert k.shape == v.shape == shape, "rows: out has another shape"
-        _lib.check(_lib.load().fhip_paged_rows(self._ref, seq, row0, rows, k.buf.ptr, v.buf.ptr, _stream_handle(stream)))
+        _lib.paged_rows(self._addr, seq, row0, rows, k.buf, v.buf, _at(stream))
         return k, v

@@ -530,10 +530,7 @@ def test_a_captured_step_serves_growing_sequences(F, paged, ty):
         c.select(q, lens, entries * R, b, nh, 4, out=outs[1], stream=stream)
         c.attention_selected(q, lens, outs[1], nh, out=outs[2], stream=stream)
 
-    # workspaces of the sizes that the capture needs, before it begins
-    need = max(lib.fhip_paged_attention_ws_bytes(caches[0]._ref, nh, entries * R), lib.fhip_paged_select_ws_bytes(caches[0]._ref, entries * R),
-               lib.fhip_paged_attention_ws_bytes(caches[0]._ref, nh, 4 * R))
-    caches[0]._workspace(need, None, s)
+    caches[0].reserve(nh, entries * R, 4, s)                     # before the capture begins
     chk(lib.fhip_stream_sync(None))
     g = F.Graph.begin(s)
     step(caches[0], bounds[0], (out, sel, some), s)

@@ -1753,6 +1753,7 @@ static int paged_attention(const char* who, const fhip_paged* kv, const float* d
     int rc = paged_view(who, kv, v);
     if (rc || (rc = paged_heads(who, kv, n_head))) return rc;
     if (!(softcap >= 0.f)) return set_error(FHIP_ERR_ARG, "%s: softcap must be >= 0", who);
+    if (kv->n_seq * n_head > 0x7FFFFFull) return set_error(FHIP_ERR_SHAPE, "%s: n_seq * n_head must be below 2^23, got %zu", who, kv->n_seq * n_head);
     if (kv->n_seq == 0) return FHIP_OK;
     if (!d_q || !d_lens || !d_out) return set_error(FHIP_ERR_ARG, "%s: NULL pointer", who);
     if (!aligned16(d_q) || !aligned16(d_out) || !aligned16(d_ws)) return set_error(FHIP_ERR_ARG, "%s: pointers must be 16-byte aligned", who);

@@ -108,11 +108,6 @@ __device__ __forceinline__ float across(float v, int lane) {
 }
 
 // ---------------------------------------------------------------- storing the rows of new tokens
-// Row i of the fused projection: + bias, RMS norm of query and key heads, rotation, queries to q_out, keys and values to the row of their page, rounded once.
-// The angle pos * base^(-2c / n_rot) is formed in f64, in turns, and only its fraction of a turn is rounded to f32: the f32 product that the contiguous
-// caches' post-processing forms is 4e-3 rad off at position 100 000.
-// A lane holds two neighbouring dims, so a wave holds 128 values (a slice): one head of 128 or two of 64. TOK tokens a workgroup: with 4 a wave has a
-// token to itself and the f64 work of its angles is shared by all of the token's heads; with 1 the waves share a token's slices.
 // values `at` and `at` + 1 of a pool; for Q8_0 the 16 lanes of a block together: d = amax / 127, codes round(v / d) half away from zero, as fhip_kvq_append's
 template <int TYPE>
 __device__ __forceinline__ void store_pair(const PagedView& kv, bool is_k, size_t at, float2 v, bool placed) {
@@ -137,6 +132,11 @@ __device__ __forceinline__ void store_pair(const PagedView& kv, bool is_k, size_
         }
     }
 }
+// Row i of the fused projection: + bias, RMS norm of query and key heads, rotation, queries to q_out, keys and values to the row of their page, rounded once.
+// The angle pos * base^(-2c / n_rot) is formed in f64, in turns, and only its fraction of a turn is rounded to f32: the f32 product that the contiguous
+// caches' post-processing forms is 4e-3 rad off at position 100 000.
+// A lane holds two neighbouring dims, so a wave holds 128 values (a slice): one head of 128 or two of 64. TOK tokens a workgroup: with 4 a wave has a
+// token to itself and the f64 work of its angles is shared by all of the token's heads; with 1 the waves share a token's slices.
 template <int TYPE, int HD, int TOK>
 __global__ __launch_bounds__(256) void append_kernel(PagedView kv, PagedPost p, int slices_per_wave) {
     constexpr int LPH = HD / 2;                       // lanes of a head
@@ -222,8 +222,10 @@ __global__ __launch_bounds__(256) void append_kernel(PagedView kv, PagedPost p, 
         for (int e = 0; e < AHEAD; e++) {
             float2 r = v[e];
             if (p.interleaved) {
-                r.x = fmaf(v[e].x, t0.x, -(v[e].y * t0.y));
-                r.y = fmaf(v[e].y, t0.x, v[e].x * t0.y);
+                if (j0 < p.n_rot) {
+                    r.x = fmaf(v[e].x, t0.x, -(v[e].y * t0.y));
+                    r.y = fmaf(v[e].y, t0.x, v[e].x * t0.y);
+                }
             } else if (half > 0) {
                 float2 o;                             // the partners
                 if (p.n_rot == HD) {                  // half a head away: 32 lanes, or 16
@@ -278,24 +280,25 @@ __global__ void bounds_kernel(PagedView kv, int hd, const uint32_t* __restrict__
     n = n < max_new ? n : max_new;
     n = n < len ? n : len;
     if (n == 0) return;
-    const uint32_t entry = ((len - n) >> kv.shift) + blockIdx.y;
-    if (entry > (len - 1) >> kv.shift) return;
-    const uint32_t page = kv.table[seq * kv.table_stride + entry];
-    if (page >= kv.n_pages) return;
-    const uint32_t start = entry << kv.shift, from = start > len - n ? start : len - n, to = len - start < R ? len : start + R;
     const int d = threadIdx.x;
-    float* b = bounds + ((size_t)page * kv.n_kv + head) * 2 * hd + d;
-    float lo = from == start ? INFINITY : b[0], hi = from == start ? -INFINITY : b[hd];
-    bool nan = lo != lo || hi != hi;
-    for (uint32_t r = from; r < to; r++) {
-        const size_t at = ((((size_t)page << kv.shift) + (r - start)) * kv.n_kv + head) * hd + d;
-        const float x = load4<TYPE>(kv.k, kv.k_scales, at & ~(size_t)3)[d & 3];
-        nan |= x != x;
-        lo = fminf(lo, x);
-        hi = fmaxf(hi, x);
+    for (uint32_t entry = ((len - n) >> kv.shift) + blockIdx.y; entry <= (len - 1) >> kv.shift; entry += gridDim.y) {
+        const uint32_t page = kv.table[seq * kv.table_stride + entry];
+        if (page >= kv.n_pages) continue;
+        const uint32_t start = entry << kv.shift, from = start > len - n ? start : len - n, to = len - start < R ? len : start + R;
+        float* b = bounds + ((size_t)page * kv.n_kv + head) * 2 * hd + d;
+        float lo = from == start ? INFINITY : b[0], hi = from == start ? -INFINITY : b[hd];
+        bool nan = lo != lo || hi != hi;
+#pragma unroll 8
+        for (uint32_t r = from; r < to; r++) {
+            const size_t at = ((((size_t)page << kv.shift) + (r - start)) * kv.n_kv + head) * hd + d;
+            const float x = load4<TYPE>(kv.k, kv.k_scales, at & ~(size_t)3)[d & 3];
+            nan |= x != x;
+            lo = fminf(lo, x);
+            hi = fmaxf(hi, x);
+        }
+        b[0] = nan ? NAN : lo;
+        b[hd] = nan ? NAN : hi;
     }
-    b[0] = nan ? NAN : lo;
-    b[hd] = nan ? NAN : hi;
 }
 
 // ---------------------------------------------------------------- the choice of pages
@@ -710,6 +713,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
         // a unit's first UNIT_COST places in the row are no steps
         const uint64_t cost = unit_cost(sp.steps);
         head = uniform((uint32_t)((at - before) / cost));
+        if (head >= (uint32_t)kv.n_kv) return;        // (lengths that change under the launch)
         unit0 = before + head * cost;
         each = per;
     }
@@ -1136,7 +1140,7 @@ __global__ __launch_bounds__(256) void join_kernel(Attend a) {
         if (threadIdx.x < HD) out[threadIdx.x] = 0.f;
         return;
     }
-    const uint32_t w0 = plan & 0x7FFFu, w1 = plan >> 15 & 0x7FFFu, second = plan >> 30;
+    const uint32_t wgs = (1u << a.log_wgs) - 1, w0 = plan & wgs, w1 = plan >> 15 & wgs, second = plan >> 30 & 1;      // (within the workspace whatever it holds)
     if (w0 == w1) return;                             // finished where it was
     auto part = [&](uint32_t w) { return a.part + ((size_t)w * 2 + (w == w0 ? second : 0)) * g * (HD + 4); };
     // a group of threads takes every GROUPS-th share; its maximum as it goes
@@ -1202,10 +1206,13 @@ namespace fhip {
 
 int launch_paged_append(uint32_t type, int hd, const PagedView& kv, const PagedPost& p, hipStream_t s) {
     const size_t slices = ((size_t)(p.n_head + 2 * kv.n_kv) * hd + 127) / 128;
-    // A wave a token once the tokens alone give every CU its waves; fewer tokens leave their slices to more waves.
-    const bool many = (size_t)p.t >= 4 * (size_t)device_cus();
-    const int each = many ? (int)slices : 1;
-    const dim3 grid(many ? (p.t + 3) / 4 : p.t, many ? 1u : (unsigned)((slices + 3) / 4));
+    // Few slices go one to a wave. From eight for each of 2048 waves on a wave takes a token's, or as many of them (eight and more) as leave MANY_WAVES. us: 999 tokens of 144
+    // heads of 64 25.0 with a slice a wave, 19.8 so; 1200 of 56 of 128 with 4096 waves 19.2, with 16384 16.6.
+    constexpr size_t MANY_WAVES = 16384;
+    const bool many = p.t * slices >= 8 * 2048;
+    const size_t most = (slices + 7) / 8, parts = many ? (p.t >= MANY_WAVES ? 1 : MANY_WAVES / p.t < most ? MANY_WAVES / p.t : most) : 1;
+    const int each = many ? (int)((slices + parts - 1) / parts) : 1;
+    const dim3 grid(many ? (p.t + 3) / 4 : p.t, many ? (unsigned)parts : (unsigned)((slices + 3) / 4));
     return by_type(type, [&](auto ty) {
         constexpr int TYPE = decltype(ty)::value;
         auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, kv, p, each); };
@@ -1217,7 +1224,7 @@ int launch_paged_append(uint32_t type, int hd, const PagedView& kv, const PagedP
 
 int launch_paged_rows(uint32_t type, int hd, const PagedView& kv, uint32_t seq, size_t row0, size_t rows, float* k_out, float* v_out, hipStream_t s) {
     const size_t width4 = (size_t)kv.n_kv * hd / 4, grid = (rows * width4 + 255) / 256;
-    if (grid > 0x7FFFFFFFull) return set_error(FHIP_ERR_SHAPE, "fhip_paged_rows: too many rows for one launch");
+    if (grid > 0xFFFFFFull) return set_error(FHIP_ERR_SHAPE, "fhip_paged_rows: too many rows for one launch");      // 2^32 threads
     return by_type(type, [&](auto ty) {
         hipLaunchKernelGGL((rows_kernel<decltype(ty)::value>), dim3((unsigned)grid, 2), dim3(256), 0, s, kv, (uint32_t)width4, seq, row0, rows, k_out, v_out);
         return check_hip(hipGetLastError(), "paged_rows launch");
@@ -1229,7 +1236,7 @@ int launch_paged_key_bounds(uint32_t type, int hd, const PagedView& kv, const ui
     uint64_t pages = ((uint64_t)max_new + R - 2) / R + 1;            // that `max_new` rows can touch
     if (pages > kv.pages_per_seq) pages = kv.pages_per_seq;
     return by_type(type, [&](auto ty) {
-        hipLaunchKernelGGL((bounds_kernel<decltype(ty)::value>), dim3(kv.n_seq * kv.n_kv, (unsigned)pages), dim3(hd), 0, s, kv, hd, lens, fresh, max_new, bounds);
+        hipLaunchKernelGGL((bounds_kernel<decltype(ty)::value>), dim3(kv.n_seq * kv.n_kv, (unsigned)(pages < 65535 ? pages : 65535)), dim3(hd), 0, s, kv, hd, lens, fresh, max_new, bounds);
         return check_hip(hipGetLastError(), "paged_key_bounds launch");
     });
 }
@@ -1275,7 +1282,6 @@ int launch_paged_attention(uint32_t type, int hd, const PagedView& kv, const flo
     const size_t units = (size_t)kv.n_seq * kv.n_kv;
     size_t keys = selected ? (size_t)n_select << kv.shift : max_len;
     if (window > 0 && (size_t)window + 31 < keys) keys = (size_t)window + 31;      // a window begins and ends within steps
-    if ((size_t)kv.n_seq * n_head > 0x7FFFFFull) return set_error(FHIP_ERR_SHAPE, "paged attention: too many sequences and heads for one launch");
     Attend a;
     a.kv = kv; a.q = q; a.lens = lens; a.selected = selected; a.out = out; a.plan = (uint32_t*)ws; a.part = ws + plan_floats(kv);
     a.max_len = max_len; a.n_select = n_select; a.window = window; a.n_head = n_head; a.softcap = softcap; a.scale = 1.0f / sqrtf((float)hd);

@@ -470,7 +470,8 @@ int fhip_paged_append(const fhip_paged* kv, const float* d_qkv, const float* d_b
  * window > 0; softcap as fhip_decode_attention_ex. out[i, h] = softmax_j(q . K_j / sqrt(head_dim)) @ V, query head h with KV head h / (n_head / n_kv), n_head a multiple of n_kv up to
  * 16 times it. d_lens is read on the device, so one captured launch serves growing sequences; max_len is the host's bound that sizes the work: a longer length is cut
  * to it and to what the table reaches. A length of 0, or no row left, gives zeros. f32 arithmetic, the rows enter as the values they stand for; the same inputs give the same bits. What lies
- * behind a sequence's last row is never part of a result, whatever it holds. d_ws: fhip_paged_attention_ws_bytes(kv, n_head, max_len) bytes of scratch, 16-byte aligned (NULL when
+ * behind a sequence's last row is never part of a result, whatever it holds; an infinite or NaN value among its rows makes what it enters non-finite (infinite values of 16-bit and Q8_0 rows make NaN). n_seq * n_head
+ * below 2^23 (FHIP_ERR_SHAPE). d_ws: fhip_paged_attention_ws_bytes(kv, n_head, max_len) bytes of scratch, 16-byte aligned (NULL when
  * that is 0), the call's own until the stream has passed it. */
 size_t fhip_paged_attention_ws_bytes(const fhip_paged* kv, size_t n_head, size_t max_len);
 int fhip_paged_attention(const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, size_t max_len, size_t n_head, size_t window, float softcap, float* d_ws,
@@ -481,12 +482,13 @@ int fhip_paged_attention(const fhip_paged* kv, const float* d_q, const uint32_t*
  * is new starts over, the others' bounds widen. No two sequences may have new rows in one page. NaN keys make NaN bounds. */
 int fhip_paged_key_bounds(const fhip_paged* kv, const uint32_t* d_lens, const uint32_t* d_new, size_t max_new, float* d_bounds, void* stream);
 /* d_selected [n_seq, n_kv, n_select]: for each sequence and KV head the first keep_first and last keep_last of its pages, then those of the highest score, the largest q . k that a key
- * within the bounds can have for any of the head's queries (formed in f64; equal ones by their place, a NaN first); as ascending indices into the sequence's row of the table, filled up with 0xFFFFFFFF.
+ * within the bounds can have for any of the head's queries (formed in f64; equal ones by their place, bounds that are not finite first); as ascending indices into the sequence's row of the table, filled up with 0xFFFFFFFF.
  * n_select at least keep_first + keep_last and 1, at most 2^20 (FHIP_ERR_SHAPE). d_ws: fhip_paged_select_ws_bytes(kv, max_len) bytes, 16-byte aligned. */
 size_t fhip_paged_select_ws_bytes(const fhip_paged* kv, size_t max_len);
 int fhip_paged_select(const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, size_t max_len, const float* d_bounds, size_t n_head, size_t n_select,
                       size_t keep_first, size_t keep_last, void* d_ws, uint32_t* d_selected, void* stream);
-/* fhip_paged_attention over the rows of the listed pages only (an index that is no page of the sequence's d_lens[i] rows is left out, each may be listed once). d_ws:
+/* fhip_paged_attention over the rows of the listed pages only, in any order, each listed once; an index that is no page of the sequence's d_lens[i] rows is left out. Of n_select entries the first as
+ * many as the sequence has pages are looked at (fhip_paged_select fills no others). d_ws:
  * fhip_paged_attention_ws_bytes(kv, n_head, n_select * page_rows) bytes. */
 int fhip_paged_attention_selected(const fhip_paged* kv, const float* d_q, const uint32_t* d_lens, const uint32_t* d_selected, size_t n_select, size_t n_head, float softcap,
                                   float* d_ws, float* d_out, void* stream);

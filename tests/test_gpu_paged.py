@@ -150,6 +150,21 @@ def test_long_sequences(F, paged, ty, n_seq, n_kv):
     check_attention(case, out, q, 4 * n_kv, lambda i: range(lens[i]))
 
 
+@typed
+@pytest.mark.parametrize("n_seq,most,window", [(150, 3000, 0), (70, 2500, 700), (300, 2000, 0), (600, 100, 0), (130, 40, 0)])
+def test_many_sequences(F, paged, ty, n_seq, most, window):
+    """More sequences than a wave has lanes, long ones among many short and empty ones; more units than the chip has workgroups and waves for."""
+    rng = np.random.default_rng(n_seq)
+    lens = [int(x) for x in rng.integers(0, 40, n_seq)]
+    for i in rng.integers(0, n_seq, 5):
+        lens[i] = int(rng.integers(most // 2, most + 1))
+    lens[-1] = most
+    case = Filled(F, paged, ty, lens, 2, 64, 16, n_seq, extra_entries=0)
+    q = (1.5 * rng.standard_normal((n_seq, 4 * 64))).astype(np.float32)
+    out = case.cache.attention(tensor(F, q), words(lens), most, 4, window=window).to_vec()
+    check_attention(case, out, q, 4, lambda i: range(max(0, lens[i] - (window or lens[i])), lens[i]))
+
+
 def test_lengths_are_cut_to_the_bound_and_to_the_table(F, paged):
     case = Filled(F, paged, P.F32, [100, 100, 40], 2, 64, 16, 9, extra_entries=0)
     q = np.random.default_rng(1).standard_normal((3, 4 * 64)).astype(np.float32)
@@ -291,6 +306,19 @@ def test_append(F, paged, ty, hd, n_kv, g, n_rot, inter, norm, bias, t):
     untouched(case, "k", written), untouched(case, "v", written)
 
 
+@pytest.mark.parametrize("inter", [False, True])
+def test_dims_behind_the_rotated_ones_pass_through(F, paged, inter):
+    """Each by itself: an infinite neighbour stays its own."""
+    hd, t = 64, 3
+    cache = paged.PagedKvCache(P.F32, 16, 1, 1, hd, 1, 1)
+    cache.set_table([[0]])
+    qkv = np.random.default_rng(2).standard_normal((t, 3 * hd)).astype(np.float32)
+    qkv[1, 41], qkv[2, 63] = np.inf, np.nan
+    q = cache.append(tensor(F, qkv), words([0] * t), words(range(t)), 1, 1e4, n_rot=32, interleaved=inter).to_vec().reshape(t, hd)
+    assert np.array_equal(bits(q[:, 32:]), bits(qkv[:, 32:64]))
+    assert np.isfinite(q[:, :32]).all()
+
+
 def test_far_positions_turn_exactly(F, paged):
     """Angles in f64: at position 4 000 000 000 an f32 product is off by whole turns."""
     hd, R = 128, 4096
@@ -393,6 +421,17 @@ def test_key_bounds_grow_with_the_rows(F, paged, ty, hd):
     used = np.concatenate([case.table[i, :-(-n // R)] for i, n in enumerate(lens)])
     rest = np.setdiff1d(np.arange(case.n_pages), used)
     assert (got[rest] == 77).all()                             # pages of nobody stay as they were
+
+
+def test_key_bounds_of_a_long_prompt(F, paged):
+    """Many pages at once, from the middle of one on."""
+    n, R = 5000, 64
+    case = Filled(F, paged, P.F16, [n], 1, 64, R, 8)
+    bounds = tensor(F, np.zeros((case.n_pages, 1, 2, 64)))
+    case.cache.key_bounds(words([37]), 37, bounds)
+    case.cache.key_bounds(words([n]), n - 37, bounds)
+    got = bounds.to_vec().reshape(case.n_pages, 1, 2, 64)
+    assert np.array_equal(got[case.table[0, :-(-n // R)]], bounds_of(case, 0, n, R).astype(np.float32))
 
 
 def test_nan_keys_make_nan_bounds_and_come_first(F, paged):

@@ -63,6 +63,7 @@ def test_arguments():
     assert attend(q=None) == ARG and attend(lens=None) == ARG and attend(out=None) == ARG and attend(q=P + 8) == ARG and attend(ws=P + 4) == ARG
     assert attend(cap=-1.0) == ARG and attend(cap=float("nan")) == ARG
     assert attend(kv=cache(n_seq=0), q=None) == OK
+    assert lib.fhip_paged_attention(cache(n_seq=65535, n_kv=64), P, P, 64, 256, 0, 0.0, P, P, None) == SHAPE and "2^23" in _lib.last_error()
     picked = lambda sel=P, n=4: lib.fhip_paged_attention_selected(kv, P, P, sel, n, 4, 0.0, P, P, None)      # noqa: E731
     assert picked(sel=None) == ARG and picked(n=0) == SHAPE and picked(n=2 ** 20 + 1) == SHAPE
     choose = lambda n=4, first=1, last=1, ws=P, b=P, out=P: lib.fhip_paged_select(kv, P, P, 64, b, 4, n, first, last, ws, out, None)      # noqa: E731

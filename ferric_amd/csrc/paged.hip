@@ -628,16 +628,6 @@ __device__ __forceinline__ Span span_of(const PagedView& kv, const uint32_t* __r
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ uint64_t uniform(uint64_t v) { return (uint64_t)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v); }
 __device__ __forceinline__ Span uniform(Span s) { return Span{uniform(s.len), uniform(s.lo), uniform(s.first), uniform(s.steps)}; }
-// Steps in front of sequence 64 b + lane in blocks of 64 sequences, and of all: a wave's scan.
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v, int lane) {      // inclusive
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t t = __shfl_up((unsigned long long)v, o);
-        if (lane >= o) v += t;
-    }
-    return v;
-}
-
 struct Attend {
     PagedView kv;
     const float* q;
@@ -655,21 +645,7 @@ struct Attend {
 // What a unit costs in steps beside its own: its queries, its first keys' trip and the waves' sums. Without it a workgroup that has many short sequences' units was the last by far: 24 sequences
 // of 1 .. 4096 keys on bf16 took 58 us where as many keys in sequences of equal length took 44.
 constexpr uint32_t UNIT_COST = 6;
-__device__ __forceinline__ uint64_t unit_cost(uint32_t steps) { return steps ? (uint64_t)steps + UNIT_COST : 0; }
-// Range of steps of a workgroup: all steps over the workgroups, `least` at least.
-__device__ __forceinline__ uint64_t places_each(uint64_t all, int log_wgs, uint32_t least) {
-    const uint64_t per = (all + ((uint64_t)1 << log_wgs) - 1) >> log_wgs;
-    return per > least ? per : least;
-}
-template <int TYPE, bool SEL>
-__device__ __forceinline__ uint64_t all_places(const Attend& a, int lane) {
-    uint64_t all = 0;
-    for (uint32_t b = 0; b < a.kv.n_seq; b += 64) {
-        const uint64_t c = b + lane < a.kv.n_seq ? unit_cost(span_of<TYPE, SEL>(a.kv, a.lens, b + lane, a.max_len, a.window, a.n_select).steps) * a.kv.n_kv : 0;
-        all += __shfl((unsigned long long)wave_scan(c, lane), 63);
-    }
-    return all;
-}
+__device__ __forceinline__ uint32_t unit_cost(uint32_t steps) { return steps ? steps + UNIT_COST : 0; }
 
 template <int TYPE, int HD, bool SEL, int WV>
 __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
@@ -683,7 +659,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
     const int g = a.n_head / kv.n_kv;
 
     // this workgroup's steps, and the unit that the first of them belongs to
-    uint64_t at = 0, end = ~0ull, unit0 = 0, each = 1;      // places [at, end) of the row of all units; unit0: the current unit's first
+    uint32_t at = 0, end = 0, unit0 = 0, each = 1;    // places [at, end) of the row of all units (the host has seen that there are fewer than 2^31); unit0: the current unit's first
     uint32_t seq = 0, head = 0, shares = 0;
     Span sp;
     if (a.log_wgs < 0) {
@@ -691,39 +667,68 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
         head = blockIdx.x % kv.n_kv;
         sp = uniform(span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select));
     } else {
-        const uint64_t all = uniform(all_places<TYPE, SEL>(a, lane)), per = places_each(all, a.log_wgs, a.min_steps);
-        at = blockIdx.x * per;
-        end = at + per < all ? at + per : all;
-        if (at >= end) return;
-        uint64_t before = 0;
-        for (uint32_t b = 0; b < kv.n_seq; b += 64) {
-            const uint64_t c = b + lane < kv.n_seq ? unit_cost(span_of<TYPE, SEL>(kv, a.lens, b + lane, a.max_len, a.window, a.n_select).steps) * kv.n_kv : 0;
-            const uint64_t upto = before + wave_scan(c, lane), here = __ballot(upto > at);
-            if (here) {
-                const int l = __builtin_ctzll(here);
-                seq = b + l;
-                before = __shfl((unsigned long long)(upto - c), l);
-                break;
-            }
-            before = __shfl((unsigned long long)upto, 63);
+        // lane l: sequence b + l, what its units cost, and what all up to it do
+        Span here;
+        uint32_t cost = 0, upto = 0;
+        auto costs = [&](uint32_t b) {
+            here = Span{0, 0, 0, 0};
+            if (b + lane < kv.n_seq) here = span_of<TYPE, SEL>(kv, a.lens, b + lane, a.max_len, a.window, a.n_select);
+            cost = unit_cost(here.steps);
+            upto = wave_upto(cost * (uint32_t)kv.n_kv);
+        };
+        uint32_t all = 0;
+        for (uint32_t b = (kv.n_seq - 1) & ~63u;; b -= 64) {      // the first 64 stay in hand
+            costs(b);
+            all += __builtin_amdgcn_readlane(upto, 63);
+            if (b == 0) break;
         }
-        seq = uniform(seq);
-        before = uniform(before);
-        sp = uniform(span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select));
-        // a unit's first UNIT_COST places in the row are no steps
-        const uint64_t cost = unit_cost(sp.steps);
-        head = uniform((uint32_t)((at - before) / cost));
-        if (head >= (uint32_t)kv.n_kv) return;        // (lengths that change under the launch)
-        unit0 = before + head * cost;
-        each = per;
+        each = (all + (1u << a.log_wgs) - 1) >> a.log_wgs;
+        each = each > a.min_steps ? each : a.min_steps;
+        at = blockIdx.x * each;
+        end = at + each < all ? at + each : all;
+        if (at >= end) return;
+        uint32_t before = 0;
+        uint64_t found;
+        while (!(found = __ballot(before + upto > at))) {
+            before += __builtin_amdgcn_readlane(upto, 63);
+            seq += 64;
+            if (seq >= kv.n_seq) return;              // (lengths that change under the launch)
+            costs(seq);
+        }
+        const int l = __builtin_ctzll(found);
+        seq += l;
+        sp = Span{(uint32_t)__builtin_amdgcn_readlane(here.len, l), (uint32_t)__builtin_amdgcn_readlane(here.lo, l), (uint32_t)__builtin_amdgcn_readlane(here.first, l),
+                  (uint32_t)__builtin_amdgcn_readlane(here.steps, l)};
+        before += __builtin_amdgcn_readlane(upto, l);
+        const uint32_t its = __builtin_amdgcn_readlane(cost, l);
+        before -= its * (uint32_t)kv.n_kv;
+        head = (at - before) / its;
+        unit0 = before + head * its;
     }
+    // to the sequence's next KV head, or the next sequence with any steps, if places of it are this workgroup's
+    auto next_unit = [&] {
+        unit0 += unit_cost(sp.steps);
+        at = unit0;
+        if (at + UNIT_COST >= end) return false;
+        if (++head == (uint32_t)kv.n_kv) {
+            head = 0;
+            do {
+                if (++seq >= kv.n_seq) return false;
+                sp = uniform(span_of<TYPE, SEL>(kv, a.lens, seq, a.max_len, a.window, a.n_select));
+            } while (sp.steps == 0);
+        }
+        return true;
+    };
 
     for (;;) {
-        // steps [from, to) of the unit are this workgroup's: those of the places [at, end)
-        auto step_at = [&](uint64_t place) { return place <= unit0 + UNIT_COST ? 0u : place - unit0 - UNIT_COST < sp.steps ? (uint32_t)(place - unit0 - UNIT_COST) : sp.steps; };
+        // steps [from, to) of the unit are this workgroup's: those of the places [at, end), of which a unit's first UNIT_COST are none
+        auto step_at = [&](uint32_t place) { return place <= unit0 + UNIT_COST ? 0u : place - unit0 - UNIT_COST < sp.steps ? place - unit0 - UNIT_COST : sp.steps; };
         const uint32_t from = step_at(at), to = a.log_wgs < 0 ? sp.steps : step_at(end);
         const bool whole = from == 0 && to == sp.steps;
-        if (to > from || a.log_wgs < 0) {
+        if (a.log_wgs >= 0 && to == from) {
+            if (!next_unit()) return;
+            continue;
+        }
         const uint32_t* table = kv.table + seq * kv.table_stride;
         const uint32_t* list = SEL ? a.selected + ((size_t)seq * kv.n_kv + head) * a.n_select : nullptr;
         const uint32_t pages = pages_of(kv, sp.len), row_values = (uint32_t)kv.n_kv * HD;
@@ -1082,7 +1087,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
         __syncthreads();
         float* part = whole ? nullptr : a.part + ((size_t)blockIdx.x * 2 + shares) * g * (HD + 4);
         if (a.log_wgs >= 0 && from == 0 && threadIdx.x == 0) {       // the unit's first steps are here: who has the others
-            const uint32_t last = whole ? blockIdx.x : (uint32_t)((unit0 + unit_cost(sp.steps) - 1) / each);
+            const uint32_t last = whole ? blockIdx.x : (unit0 + unit_cost(sp.steps) - 1) / each;
             a.plan[seq * kv.n_kv + head] = (uint32_t)blockIdx.x | last << 15 | shares << 30;
         }
         shares += !whole;
@@ -1107,19 +1112,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                 if (d == 0) { part[g * HD + 2 * h] = top; part[g * HD + 2 * h + 1] = sum; }
             }
         }
-        }
-        if (a.log_wgs < 0) return;
-        // the next unit: the sequence's next KV head, or the next sequence with any steps
-        unit0 += unit_cost(sp.steps);
-        at = unit0;
-        if (at + UNIT_COST >= end) return;
-        if (++head == (uint32_t)kv.n_kv) {
-            head = 0;
-            do {
-                if (seq + 1 >= kv.n_seq) return;
-                sp = uniform(span_of<TYPE, SEL>(kv, a.lens, ++seq, a.max_len, a.window, a.n_select));
-            } while (sp.steps == 0);
-        }
+        if (a.log_wgs < 0 || !next_unit()) return;
         __syncthreads();
     }
 }
@@ -1271,6 +1264,7 @@ constexpr int LOG_WGS = 9, MIN_STEPS = 6;
 // 64 of 500 28.6 | 33.2, 64 of 2000 97.9 | 103, but 8 of 2000 24.5 | 20.1.
 static bool own_workgroups(uint32_t type, const PagedView& kv, size_t keys) {
     const size_t steps = (keys + (type == FHIP_F32 ? 15 : 31)) / (type == FHIP_F32 ? 16 : 32);
+    if ((steps + UNIT_COST) * kv.n_seq * kv.n_kv >= (size_t)1 << 31) return true;      // the deal counts in 32 bits
     return steps <= 16 || ((size_t)kv.n_seq * kv.n_kv >= ((size_t)1 << LOG_WGS) && steps <= 64);
 }
 static size_t plan_floats(const PagedView& kv) { return ((size_t)kv.n_seq * kv.n_kv + 3) / 4 * 4; }
@@ -1280,12 +1274,13 @@ size_t paged_attention_ws_bytes(uint32_t type, const PagedView& kv, int hd, int 
 int launch_paged_attention(uint32_t type, int hd, const PagedView& kv, const float* q, const uint32_t* lens, uint32_t max_len, const uint32_t* selected, uint32_t n_select,
                            int n_head, uint32_t window, float softcap, float* ws, float* out, hipStream_t s) {
     const size_t units = (size_t)kv.n_seq * kv.n_kv;
-    size_t keys = selected ? (size_t)n_select << kv.shift : max_len;
+    const size_t bound = selected ? (size_t)n_select << kv.shift : max_len;
+    size_t keys = bound;
     if (window > 0 && (size_t)window + 31 < keys) keys = (size_t)window + 31;      // a window begins and ends within steps
     Attend a;
     a.kv = kv; a.q = q; a.lens = lens; a.selected = selected; a.out = out; a.plan = (uint32_t*)ws; a.part = ws + plan_floats(kv);
     a.max_len = max_len; a.n_select = n_select; a.window = window; a.n_head = n_head; a.softcap = softcap; a.scale = 1.0f / sqrtf((float)hd);
-    a.log_wgs = own_workgroups(type, kv, keys) ? -1 : LOG_WGS;
+    a.log_wgs = own_workgroups(type, kv, keys) || own_workgroups(type, kv, bound) ? -1 : LOG_WGS;      // (the latter: the caller may have no workspace)
     a.min_steps = MIN_STEPS;
     const bool alone = a.log_wgs < 0 && units > 4 * (size_t)device_cus();      // more units than the chip has waves for by fours: a wave each
     const dim3 grid(a.log_wgs < 0 ? (unsigned)units : 1u << LOG_WGS);

@@ -68,12 +68,12 @@ class PagedKvCache:
         the stream may name it. Graphs that may run at the same time need workspaces of their own."""
         if ws is not None:
             return ws
-        at = n_heads, keys.bit_length()               # sized for the next power of two: asked for once
-        need = self._needs.get(at)
+        need = self._needs.get((n_heads, keys))
         if need is None:
             lib = _lib.load()
-            need = lib.fhip_paged_attention_ws_bytes(self._ref, n_heads, 1 << at[1]) if n_heads else lib.fhip_paged_select_ws_bytes(self._ref, 1 << at[1])
-            self._needs[at] = need
+            if len(self._needs) > 1000:               # sizes of lengths that are past
+                self._needs.clear()
+            need = self._needs[n_heads, keys] = lib.fhip_paged_attention_ws_bytes(self._ref, n_heads, keys) if n_heads else lib.fhip_paged_select_ws_bytes(self._ref, keys)
         if need == 0:
             return None
         kept = self._ws.setdefault(None if stream is None else stream.handle.value, [])

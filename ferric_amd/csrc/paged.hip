@@ -310,52 +310,68 @@ __device__ __forceinline__ uint64_t order_key(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     return b >> 63 ? ~b : b | 1ull << 63;
 }
-// On v_mfma_f64_16x16x4_f64: 16 pages by the head's queries, max(q, 0) and min(q, 0) in f64 in LDS as the instructions take them, a lane's bounds four neighbouring dims of a page at a
-// time. Bound by the bounds' bytes: the instructions of 16 pages take 4096 cycles, 9.8 TB/s of bounds on the chip. us for 24 sequences' 52 MB of bounds: a wave a page, with a sum over its lanes for each
-// query, 75; with the queries in every wave's registers, two waves a SIMD, 24.5; so 20.
-template <int HD>
+// On v_mfma_f64_4x4x4_4b_f64, four blocks of 4 pages by 4 queries each: CALLS of them for up to 4 CALLS queries, max(q, 0) and min(q, 0) in f64 in LDS, a lane's bounds four neighbouring dims of
+// a page at a time. Bound by the bounds' bytes; the instructions of 16 pages take 1024 CALLS cycles (CALLS = 2: 19.7 TB/s of bounds on the chip). us for 24 sequences' 52 MB of bounds: a wave a page, with a sum over its
+// lanes for each of 8 queries, 75; on the 16 x 16 x 4 instruction, whose 16 columns take 4096 cycles whatever is in them, 20; this 18, half of the copy rate: the pages' kilobytes lie
+// anywhere, and their trip of 2 us is most of a wave's life.
+template <int HD, int CALLS>
 __global__ __launch_bounds__(256) void score_kernel(PagedView kv, const float* __restrict__ q, const uint32_t* __restrict__ lens, uint32_t max_len, const float* __restrict__ bounds,
                                                     int n_head, uint32_t first, uint32_t last, uint64_t* __restrict__ keys, uint32_t key_stride) {
     constexpr int NI = HD / 16;
-    __shared__ double up[4 * NI][64], down[4 * NI][64];
+    __shared__ double up[CALLS][4 * NI][16], down[CALLS][4 * NI][16];      // [..][dim 16 i + 4 k + e as 4 i + e][4 k + query % 4]
     const int lane = threadIdx.x & 63, n = lane & 15, kg = lane >> 4, g = n_head / kv.n_kv, head = blockIdx.y;
     const uint32_t seq = blockIdx.z, pages = pages_of(kv, rows_of(kv, lens, seq, max_len)), groups = (pages + 15) / 16;
     if (blockIdx.x * 4 >= groups) return;
-    uint32_t j = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t j = blockIdx.x * 4 + (threadIdx.x >> 6);
     const uint32_t* table = kv.table + seq * kv.table_stride;
     keys += ((size_t)seq * kv.n_kv + head) * key_stride;
-    uint32_t mine = j < groups && 16 * j + n < pages ? table[16 * j + n] : NO_PAGE;
-    const float* qh = q + ((size_t)seq * n_head + head * g + (n < g ? n : 0)) * HD + 4 * kg;
+    const uint32_t mine = j < groups && 16 * j + n < pages ? table[16 * j + n] : NO_PAGE;
+    const float* b = bounds + ((size_t)(mine < kv.n_pages ? mine : 0) * kv.n_kv + head) * 2 * HD + 4 * kg;
+    f32x4 lo[NI], hi[NI];
 #pragma unroll
-    for (int i = threadIdx.x >> 6; i < NI; i += 4) {
-        const f32x4 x = *(const f32x4*)(qh + 16 * i);
+    for (int i = 0; i < NI; i++) {
+        lo[i] = *(const f32x4*)(b + 16 * i);
+        hi[i] = *(const f32x4*)(b + HD + 16 * i);
+    }
+    __builtin_amdgcn_sched_barrier(0);                // all on their way while the queries are laid out
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            up[4 * i + e][lane] = x[e] < 0.f ? 0.0 : (double)x[e];      // (no number stays one)
-            down[4 * i + e][lane] = x[e] < 0.f ? (double)x[e] : 0.0;
-        }
+    for (int t = threadIdx.x; t < CALLS * 4 * HD; t += 256) {
+        const int query = t / HD, dim = t % HD;
+        const float x = query < g ? q[((size_t)seq * n_head + head * g + query) * HD + dim] : 0.f;
+        const int at = 4 * (dim / 16) + dim % 4, slot = dim / 4 % 4 * 4 + query % 4;
+        up[query / 4][at][slot] = x < 0.f ? 0.0 : (double)x;      // (no number stays one)
+        down[query / 4][at][slot] = x < 0.f ? (double)x : 0.0;
     }
     __syncthreads();
     if (j >= groups) return;
-    const float* b = bounds + ((size_t)(mine < kv.n_pages ? mine : 0) * kv.n_kv + head) * 2 * HD + 4 * kg;
-    f64x4 s = (f64x4){0, 0, 0, 0}, s2 = s;
+    double s[CALLS], s2[CALLS];
 #pragma unroll
-    for (int i = 0; i < NI; i++) {
-        const f32x4 lo = *(const f32x4*)(b + 16 * i), hi = *(const f32x4*)(b + HD + 16 * i);
+    for (int c = 0; c < CALLS; c++) s[c] = s2[c] = 0;
+    const int slot = 4 * kg + (n & 3);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            s = __builtin_amdgcn_mfma_f64_16x16x4f64((double)hi[e], up[4 * i + e][lane], s, 0, 0, 0);
-            s2 = __builtin_amdgcn_mfma_f64_16x16x4f64((double)lo[e], down[4 * i + e][lane], s2, 0, 0, 0);
-        }
+    for (int i = 0; i < NI; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int c = 0; c < CALLS; c++) {
+                s[c] = __builtin_amdgcn_mfma_f64_4x4x4f64((double)hi[i][e], up[c][4 * i + e][slot], s[c], 0, 0, 0);
+                s2[c] = __builtin_amdgcn_mfma_f64_4x4x4f64((double)lo[i][e], down[c][4 * i + e][slot], s2[c], 0, 0, 0);
+            }
+    // page 16 j + n / 4 * 4 + kg, query 4 c + n % 4
+    const int row = (n & ~3) + kg;
+    const bool there = __shfl(mine, row) < kv.n_pages;
+    uint64_t key = order_key(-INFINITY);
+#pragma unroll
+    for (int c = 0; c < CALLS; c++) {
+        const uint64_t k = order_key(s[c] + s2[c]);
+        if (there && 4 * c + (n & 3) < g && k > key) key = k;
     }
-#pragma unroll
-    for (int r = 0; r < 4; r++) {                     // page 16 j + 4 r + kg, query n
-        const uint32_t page = 16 * j + 4 * r + kg;
-        const bool there = __shfl(mine, 4 * r + kg) < kv.n_pages;
-        uint64_t key = n < g && there ? order_key(s[r] + s2[r]) : order_key(-INFINITY);
-        key = row16(key, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-        if (n == 0 && page < pages) keys[page] = page < first || page + last >= pages ? ~0ull : key;
-    }
+    const uint64_t a = dpp<0xB1>(key);                // over the four queries
+    key = a > key ? a : key;
+    const uint64_t c = dpp<0x4E>(key);
+    key = c > key ? c : key;
+    const uint32_t page = 16 * j + row;
+    if ((n & 3) == 0 && page < pages) keys[page] = page < first || page + last >= pages ? ~0ull : key;
 }
 
 // The n_select largest keys of a list, equal ones by their place, as ascending places. One workgroup a list. The key that the last chosen one has is found by counting: the
@@ -1255,8 +1271,10 @@ int launch_paged_select(int hd, const PagedView& kv, const float* q, const uint3
     const uint32_t pages = pages_at_most(kv, max_len);
     if (pages > 0) {
         const dim3 grid((pages + 63) / 64, kv.n_kv, kv.n_seq);
-        if (hd == 128) hipLaunchKernelGGL((score_kernel<128>), grid, dim3(256), 0, s, kv, q, lens, max_len, bounds, n_head, first, last, (uint64_t*)ws, pages);
-        else hipLaunchKernelGGL((score_kernel<64>), grid, dim3(256), 0, s, kv, q, lens, max_len, bounds, n_head, first, last, (uint64_t*)ws, pages);
+        const int calls = (n_head / kv.n_kv + 3) / 4;
+        auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, kv, q, lens, max_len, bounds, n_head, first, last, (uint64_t*)ws, pages); };
+        if (hd == 128) calls == 1 ? go(score_kernel<128, 1>) : calls == 2 ? go(score_kernel<128, 2>) : calls == 3 ? go(score_kernel<128, 3>) : go(score_kernel<128, 4>);
+        else calls == 1 ? go(score_kernel<64, 1>) : calls == 2 ? go(score_kernel<64, 2>) : calls == 3 ? go(score_kernel<64, 3>) : go(score_kernel<64, 4>);
     }
     const dim3 lists(kv.n_seq * kv.n_kv);
     auto go = [&](auto kernel, int threads) {

@@ -19,7 +19,6 @@ using fhip::PagedPost;
 using fhip::PagedView;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef double f64x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -312,8 +311,8 @@ __device__ __forceinline__ uint64_t order_key(double v) {
 }
 // On v_mfma_f64_4x4x4_4b_f64, four blocks of 4 pages by 4 queries each: CALLS of them for up to 4 CALLS queries, max(q, 0) and min(q, 0) in f64 in LDS, a lane's bounds four neighbouring dims of
 // a page at a time. Bound by the bounds' bytes; the instructions of 16 pages take 1024 CALLS cycles (CALLS = 2: 19.7 TB/s of bounds on the chip). us for 24 sequences' 52 MB of bounds: a wave a page, with a sum over its
-// lanes for each of 8 queries, 75; on the 16 x 16 x 4 instruction, whose 16 columns take 4096 cycles whatever is in them, 20; this 18, half of the copy rate: the pages' kilobytes lie
-// anywhere, and their trip of 2 us is most of a wave's life.
+// lanes for each of 8 queries, 75; on the 16 x 16 x 4 instruction, whose 16 columns take 4096 cycles whatever is in them, 20; this 18 to 19.5, 2.7 TB/s: waves
+// wait for more than half of their cycles.
 template <int HD, int CALLS>
 __global__ __launch_bounds__(256) void score_kernel(PagedView kv, const float* __restrict__ q, const uint32_t* __restrict__ lens, uint32_t max_len, const float* __restrict__ bounds,
                                                     int n_head, uint32_t first, uint32_t last, uint64_t* __restrict__ keys, uint32_t key_stride) {
@@ -587,8 +586,8 @@ __device__ __forceinline__ void cut(float a, float b, uint32_t (&w)[3]) {
 }
 
 // tanh of four scores over their cap, which is small for nearly all of them: its series up to y^17 within 1/2 (what is left out is 3e-10 of it there), otherwise 1 - 2 / (1 + e^2y), whose
-// cancellation costs a factor of two there at most. The library's tanhf, two branches a value that a wave takes both, was half of a capped launch: 33 sequences, window 1024,
-// 16 heads of 64 on Q8_0 81.7 us a pass with it.
+// cancellation costs a factor of two there at most. The library's tanhf has two branches a value, and a wave takes both: the kernel for 33 sequences, window
+// 1024, 16 heads of 64 on Q8_0 took 74.5 us with it and 69.2 with this and the bookkeeping in scalar registers.
 __device__ __forceinline__ f32x4 tanh4(f32x4 y) {
     const f32x4 z = y * y;
     f32x4 t = z * (6404582.f / 10854718875.f) - 929569.f / 638512875.f;
@@ -664,8 +663,8 @@ constexpr uint32_t UNIT_COST = 6;
 __device__ __forceinline__ uint32_t unit_cost(uint32_t steps) { return steps ? steps + UNIT_COST : 0; }
 
 // Workgroups go round the eight XCDs, each with an L2 of its own. Place of workgroup b of n so that those of an XCD are neighbours: for Q8_0, whose rows' scales are a line for all KV heads of a sequence.
-// us with it | without: a window of 33 sequences, 16 heads of 64, 26.5 | 28.3; 8 of 2000 keys 19.7 | 20.4; the other types, whose heads share nothing, are 2 .. 5 % faster spread out (64 of 2000 on
-// bf16 100 | 97).
+// us with it | without: a window of 33 sequences, 16 heads of 64, 26.5 | 28.3; 8 of 2000 keys 19.7 | 20.4; the other types, whose heads share nothing, are up to 10 % faster spread out (64 of 2000 on
+// bf16 100 | 97, 8 of 4096 on f32 60 | 55), but for one of 131072 on bf16, 104.5 | 107.6.
 __device__ __forceinline__ uint32_t xcd_neighbours(uint32_t b, uint32_t n) {
     const uint32_t x = b % 8, each = n / 8, more = n % 8;
     return x * each + (x < more ? x : more) + b / 8;

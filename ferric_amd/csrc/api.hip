@@ -1720,6 +1720,10 @@ static int paged_heads(const char* who, const fhip_paged* kv, size_t n_head) {
         return set_error(FHIP_ERR_SHAPE, "%s: n_head must be a multiple of n_kv up to 16 times it, got %zu over %zu", who, n_head, kv->n_kv);
     return FHIP_OK;
 }
+static int paged_lists(const char* who, const fhip_paged* kv) {      // a workgroup of up to 1024 threads for each, of which a launch has less than 2^32
+    if (kv->n_seq * kv->n_kv >= (1u << 22)) return set_error(FHIP_ERR_SHAPE, "%s: n_seq * n_kv must be below 2^22, got %zu", who, kv->n_seq * kv->n_kv);
+    return FHIP_OK;
+}
 static uint32_t paged_bound(size_t n) { return n < 0xFFFFFFFFull ? (uint32_t)n : 0xFFFFFFFFu; }
 
 int fhip_paged_append(const fhip_paged* kv, const float* d_qkv, const float* d_bias, const float* d_q_norm, const float* d_k_norm, const uint32_t* d_seqs,
@@ -1729,7 +1733,7 @@ int fhip_paged_append(const fhip_paged* kv, const float* d_qkv, const float* d_b
     int rc = paged_view("fhip_paged_append", kv, v);
     if (rc || (rc = paged_heads("fhip_paged_append", kv, n_head)) || (rc = rope_checks("fhip_paged_append", n_head + 2 * kv->n_kv, kv->head_dim, n_rot))) return rc;
     if (t == 0) return FHIP_OK;
-    if (t > 0x7FFFFFFFull) return set_error(FHIP_ERR_SHAPE, "fhip_paged_append: more than 2^31 - 1 tokens");
+    if (t > (1u << 25)) return set_error(FHIP_ERR_SHAPE, "fhip_paged_append: more than 2^25 tokens");      // a launch has less than 2^32 threads
     if (n_rot > 0 && !(base > 0.f)) return set_error(FHIP_ERR_ARG, "fhip_paged_append: base must be > 0");
     if (!d_qkv || !d_positions || !d_q_out) return set_error(FHIP_ERR_ARG, "fhip_paged_append: NULL pointer");
     if (!aligned16(d_qkv) || !aligned16(d_q_out) || !aligned16(d_bias) || !aligned16(d_q_norm) || !aligned16(d_k_norm))
@@ -1783,7 +1787,7 @@ int fhip_paged_attention_selected(const fhip_paged* kv, const float* d_q, const 
 int fhip_paged_key_bounds(const fhip_paged* kv, const uint32_t* d_lens, const uint32_t* d_new, size_t max_new, float* d_bounds, void* stream) {
     fhip::PagedView v;
     int rc = paged_view("fhip_paged_key_bounds", kv, v);
-    if (rc) return rc;
+    if (rc || (rc = paged_lists("fhip_paged_key_bounds", kv))) return rc;
     if (kv->n_seq == 0 || kv->pages_per_seq == 0 || max_new == 0) return FHIP_OK;
     if (!d_lens || !d_bounds) return set_error(FHIP_ERR_ARG, "fhip_paged_key_bounds: NULL pointer");
     if ((rc = need_init())) return rc;
@@ -1799,7 +1803,7 @@ int fhip_paged_select(const fhip_paged* kv, const float* d_q, const uint32_t* d_
                       size_t keep_first, size_t keep_last, void* d_ws, uint32_t* d_selected, void* stream) {
     fhip::PagedView v;
     int rc = paged_view("fhip_paged_select", kv, v);
-    if (rc || (rc = paged_heads("fhip_paged_select", kv, n_head)) || (rc = select_count("fhip_paged_select", n_select))) return rc;
+    if (rc || (rc = paged_heads("fhip_paged_select", kv, n_head)) || (rc = select_count("fhip_paged_select", n_select)) || (rc = paged_lists("fhip_paged_select", kv))) return rc;
     if (keep_first > n_select || keep_last > n_select - keep_first)
         return set_error(FHIP_ERR_SHAPE, "fhip_paged_select: keep_first %zu and keep_last %zu exceed n_select %zu", keep_first, keep_last, n_select);
     if (kv->n_seq == 0) return FHIP_OK;

@@ -461,7 +461,8 @@ typedef struct fhip_paged {
  * heads rounded once (to nearest, ties to even; Q8_0 as fhip_kvq_append rounds) to their row. Token i is row d_positions[i] of sequence d_seqs[i] (NULL: of sequence i); one that the
  * table or d_seqs has no place for leaves its query only. No two tokens of a call may have the same place. n_head is a multiple of n_kv, up to 16 times it.
  * The angle position * base^(-2c / n_rot) [* d_freq_scale[c]] is formed in f64 (fhip_qkv_post rounds the frequency and the product to f32, 4e-3 rad at position 100 000), so rows differ
- * from its rows by that. A token's row has the same bits in every batch. Pointers 16-byte aligned; d_q_out may not overlap d_qkv. t = 0: nothing is done. */
+ * from its rows by that. A token's row has the same bits in every batch. Pointers 16-byte aligned; d_q_out may not overlap d_qkv. t = 0: nothing is done; at most
+ * 2^25 tokens (FHIP_ERR_SHAPE). */
 int fhip_paged_append(const fhip_paged* kv, const float* d_qkv, const float* d_bias, const float* d_q_norm, const float* d_k_norm, const uint32_t* d_seqs,
                       const uint32_t* d_positions, const float* d_freq_scale, size_t t, size_t n_head, size_t n_rot, int interleaved, float eps, float base,
                       float* d_q_out, void* stream);
@@ -479,7 +480,8 @@ int fhip_paged_attention(const fhip_paged* kv, const float* d_q, const uint32_t*
 
 /* Sparse attention over the pages whose keys promise most. d_bounds [n_pages, n_kv, 2, head_dim]: smallest and largest value of each dim among a page's keys, kept up to date
  * by the caller's calls of fhip_paged_key_bounds behind its appends: the last d_new[i] rows of sequence i (NULL: max_new; never more than max_new or d_lens[i]) are new, a page whose first row
- * is new starts over, the others' bounds widen. No two sequences may have new rows in one page. NaN keys make NaN bounds. */
+ * is new starts over, the others' bounds widen. No two sequences may have new rows in one page. NaN keys make NaN bounds. n_seq * n_kv below 2^22, here
+ * and for fhip_paged_select (FHIP_ERR_SHAPE). */
 int fhip_paged_key_bounds(const fhip_paged* kv, const uint32_t* d_lens, const uint32_t* d_new, size_t max_new, float* d_bounds, void* stream);
 /* d_selected [n_seq, n_kv, n_select]: for each sequence and KV head the first keep_first and last keep_last of its pages, then those of the highest score, the largest q . k that a key
  * within the bounds can have for any of the head's queries (formed in f64; equal ones by their place, bounds that are not finite first); as ascending indices into the sequence's row of the table, filled up with 0xFFFFFFFF.

@@ -81,3 +81,11 @@ def test_without_a_device_a_good_call_says_so():
         pytest.skip("device already initialised in this process")
     for got in calls(cache()):
         assert got == ARG and "fhip_init" in _lib.last_error()
+
+
+def test_launches_of_more_than_2_32_threads():
+    lib = _lib.load()
+    assert lib.fhip_paged_append(cache(), P, None, None, None, None, P, None, 2 ** 25 + 1, 4, 64, 0, 1e-6, 1e4, P, None) == SHAPE and "2^25" in _lib.last_error()
+    many = cache(n_seq=65535, n_kv=4096)
+    assert lib.fhip_paged_select(many, P, P, 64, P, 4096, 4, 1, 1, P, P, None) == SHAPE and "2^22" in _lib.last_error()
+    assert lib.fhip_paged_key_bounds(many, P, None, 1, P, None) == SHAPE and "2^22" in _lib.last_error()

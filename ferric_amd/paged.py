@@ -66,14 +66,15 @@ class PagedKvCache:
     def _workspace(self, n_heads, keys, ws, stream):
         """The caller's workspace, or one kept for the stream, for attention over `keys` keys a sequence (n_heads 0: for select). What was outgrown stays: a graph captured on
         the stream may name it. Graphs that may run at the same time need workspaces of their own."""
-        if ws is not None:
-            return ws
         need = self._needs.get((n_heads, keys))
         if need is None:
             lib = _lib.load()
             if len(self._needs) > 1000:               # sizes of lengths that are past
                 self._needs.clear()
             need = self._needs[n_heads, keys] = lib.fhip_paged_attention_ws_bytes(self._ref, n_heads, keys) if n_heads else lib.fhip_paged_select_ws_bytes(self._ref, keys)
+        if ws is not None:
+            assert getattr(ws, "nbytes", need) >= need, f"a workspace of {ws.nbytes} bytes, {need} are needed"
+            return ws
         if need == 0:
             return None
         kept = self._ws.setdefault(None if stream is None else stream.handle.value, [])

@@ -89,3 +89,22 @@ def test_launches_of_more_than_2_32_threads():
     many = cache(n_seq=65535, n_kv=4096)
     assert lib.fhip_paged_select(many, P, P, 64, P, 4096, 4, 1, 1, P, P, None) == SHAPE and "2^22" in _lib.last_error()
     assert lib.fhip_paged_key_bounds(many, P, None, 1, P, None) == SHAPE and "2^22" in _lib.last_error()
+
+
+def test_a_workspace_that_is_too_small(monkeypatch):
+    from types import SimpleNamespace as N
+
+    from ferric_amd import paged
+    from ferric_amd.qmatrix import Tensor
+    monkeypatch.setattr(_lib, "init", lambda *a: None)
+    at = N(ptr=P)
+    kv = paged.PagedKvCache.wrap(0, 16, 64, 2, 64, at, at, None, None, at, 1, 64)
+    few, none = N(ptr=P, nbytes=16), N(ptr=P, nbytes=0)
+    row, lens, bounds = Tensor(at, (1, 256)), Tensor(at, (1,)), Tensor(at, (64, 2, 2, 64))
+    with pytest.raises(AssertionError, match="workspace of 16 bytes"):
+        kv.attention(row, lens, 1024, 4, out=row, ws=few)
+    with pytest.raises(AssertionError, match="workspace of 16 bytes"):
+        kv.select(row, lens, 1024, bounds, 4, 4, out=Tensor(at, (1, 2, 4)), ws=few)
+    with pytest.raises(AssertionError, match="workspace of 16 bytes"):
+        kv.attention_selected(row, lens, Tensor(at, (1, 2, 40)), 4, out=row, ws=few)
+    assert kv._workspace(4, 100, none, None) is none            # short: needs none

@@ -310,9 +310,9 @@ __device__ __forceinline__ uint64_t order_key(double v) {
     return b >> 63 ? ~b : b | 1ull << 63;
 }
 // On v_mfma_f64_4x4x4_4b_f64, four blocks of 4 pages by 4 queries each: CALLS of them for up to 4 CALLS queries, max(q, 0) and min(q, 0) in f64 in LDS, a lane's bounds four neighbouring dims of
-// a page at a time. Bound by the bounds' bytes; the instructions of 16 pages take 1024 CALLS cycles (CALLS = 2: 19.7 TB/s of bounds on the chip). us for 24 sequences' 52 MB of bounds: a wave a page, with a sum over its
-// lanes for each of 8 queries, 75; on the 16 x 16 x 4 instruction, whose 16 columns take 4096 cycles whatever is in them, 20; this 18 to 19.5, 2.7 TB/s: waves
-// wait for more than half of their cycles.
+// a page at a time. The bounds' bytes are the floor; the instructions of 16 pages take 1024 CALLS cycles (CALLS = 2: 19.7 TB/s of bounds on the chip). us for 24 sequences' 52 MB of bounds: a wave a page, with a sum over its
+// lanes for each of 8 queries, 75; on the 16 x 16 x 4 instruction, whose 16 columns take 4096 cycles whatever is in them, 20; this 18 to 19.5, 2.7 TB/s: of the
+// waves' cycles 46 % count as SQ_WAIT_ANY and 43 % as SQ_WAIT_INST_ANY.
 template <int HD, int CALLS>
 __global__ __launch_bounds__(256) void score_kernel(PagedView kv, const float* __restrict__ q, const uint32_t* __restrict__ lens, uint32_t max_len, const float* __restrict__ bounds,
                                                     int n_head, uint32_t first, uint32_t last, uint64_t* __restrict__ keys, uint32_t key_stride) {

@@ -32,6 +32,7 @@ struct Elem {
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2)); }   // to nearest, ties to even
@@ -538,8 +539,10 @@ __global__ __launch_bounds__(T) void select_kernel(PagedView kv, const uint32_t*
 //   bf16   v_mfma_f32_16x16x32_bf16; q and p as three bf16 values each, cut off rather than rounded, so that they add up to the f32 value.
 //   f16    v_mfma_f32_16x16x32_f16; q (times a power of two that brings its largest value to 2^14) and p (times 2^15) as two f16 values, 22 bits.
 //   Q8_0   keys as f16 holds their codes, q as for f16, a block of 32 dims an instruction, whose sum is multiplied by the block's scale; values c * d, 8 by 11 bits, as the two f16 values
-//          whose sum they are, p times 2^7 as two (three products: the two small parts' is 2^-22 of the result). On the f32 instruction, which takes four keys where
+//          whose sum they are, p times 2^15 as two (three products: the two small parts' is 2^-22 of the result). On the f32 instruction, which takes four keys where
 //          these take 32, a capped window of 33 sequences, 16 heads of 64, took 69 us.
+// A step that f16 cannot hold, which a scale of 512 and more makes of Q8_0 values, takes values and weights as three bf16 values each. us, such a scale in every step | in none: Q8_0, 64 sequences
+// of 2000 keys, 8 KV heads of 128 with 5 queries 91 | 62, one of 65536 with 8 queries 57 | 39.
 // Bound by the rows' bytes. The next step's keys are requested once the current ones are multiplied, its values once the current ones are: eight waves a CU keep 64 KB and more
 // on the way without a second set of registers.
 //
@@ -617,6 +620,7 @@ struct Path {
     static constexpr int KEYS = 16 * TILES;
     static constexpr int PARTS = TYPE == FHIP_BF16 ? 3 : 2;
     static constexpr bool HALF = TYPE != FHIP_F32;                    // on a 16-bit instruction
+    static constexpr float UP = TYPE == FHIP_F16 || TYPE == FHIP_Q8_0 ? 32768.f : 1.f;      // of the weights
 };
 
 // Keys of sequence `seq` that are attended to, [lo, len), and the steps that they lie in.
@@ -1020,30 +1024,57 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                 }
             // weighted rows
             if constexpr (P::HALF) {
-                float up = TYPE == FHIP_F16 ? 32768.f : TYPE == FHIP_Q8_0 ? 128.f : 1.f;
-                uint32_t d2[TYPE == FHIP_Q8_0 ? 4 : 1];      // Q8_0: the scales of keys 2 x and 2 x + 1 in the lane's order
-                if constexpr (TYPE == FHIP_Q8_0) {
-                    uint32_t big = 0;
+                // p as PARTS 16-bit values each
+                auto cut_weights = [&](auto bf, auto& pp) {
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
-                        const uint16_t u = vd[x / 2][2 * (x & 1)], w = vd[x / 2][2 * (x & 1) + 1];
-                        d2[x] = (uint32_t)u | (uint32_t)w << 16;
-                        big |= (u > 0x5FFFu) | (w > 0x5FFFu);      // 512 and more (or no number): c * d would leave f16
-                    }
-                    if (__any(big)) {                 // a 256th of the scales, 256 times the weights
-                        up = 32768.f;
+                        uint32_t w[3];
+                        cut<bf()>(p[x / 2][2 * (x & 1)] * P::UP, p[x / 2][2 * (x & 1) + 1] * P::UP, w);
 #pragma unroll
-                        for (int x = 0; x < 4; x++) d2[x] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, d2[x]) * (f16x2){(_Float16)(1.f / 256.f), (_Float16)(1.f / 256.f)});
+                        for (int e = 0; e < (int)(sizeof(pp) / sizeof(Frag)); e++) pp[e].w[x] = w[e];
+                    }
+                };
+                uint32_t d2[TYPE == FHIP_Q8_0 ? 4 : 1];      // Q8_0: the scales of keys 2 x and 2 x + 1 in the lane's order
+                if constexpr (TYPE == FHIP_Q8_0) {
+                    u16x2 most = {0, 0};
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        d2[x] = (uint32_t)vd[x / 2][2 * (x & 1)] | (uint32_t)vd[x / 2][2 * (x & 1) + 1] << 16;
+                        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, d2[x]));
+                    }
+                    if (__any(most.x > 0x5FFFu || most.y > 0x5FFFu)) {      // 512 and more (or no number): c * d would leave f16
+                        // Values and weights as three bf16 values each, which have f32's range: all of their products but that of the smallest (2^-30 of the whole).
+                        Frag pp[3];
+                        cut_weights(std::true_type(), pp);
+#pragma unroll
+                        for (int j = 0; j < NJ; j++) {
+                            float v[8];               // of the lane's keys
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                const f16x2 d = __builtin_bit_cast(f16x2, d2[e / 2]);
+                                v[e] = (float)(int8_t)(vr[e / 4][e % 4][j / 4] >> 8 * (j % 4)) * (float)(e & 1 ? d.y : d.x);
+                            }
+#pragma unroll
+                            for (int b = 0; b < 3; b++) {
+                                Frag f;
+#pragma unroll
+                                for (int x = 0; x < 4; x++) f.w[x] = upper_halves(__float_as_uint(v[2 * x]), __float_as_uint(v[2 * x + 1]));
+#pragma unroll
+                                for (int e = b < 2 ? 2 : 1; e >= 0; e--) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.b, pp[e].b, acc[j], 0, 0, 0);
+#pragma unroll
+                                for (int e = 0; e < 8; e++) v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
+                            }
+                        }
+                        // and nothing is left for the other way (as one of two ways it would cost every step a fifth more registers)
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            d2[x] = 0;
+                            p[x / 2][2 * (x & 1)] = p[x / 2][2 * (x & 1) + 1] = 0.f;
+                        }
                     }
                 }
                 Frag pp[PARTS];
-#pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    uint32_t w[3];
-                    cut<TYPE == FHIP_BF16>(p[x / 2][2 * (x & 1)] * up, p[x / 2][2 * (x & 1) + 1] * up, w);
-#pragma unroll
-                    for (int e = 0; e < PARTS; e++) pp[e].w[x] = w[e];
-                }
+                cut_weights(std::integral_constant<bool, TYPE == FHIP_BF16>(), pp);
 #pragma unroll
                 for (int j = 0; j < NJ; j++) {
                     Frag f, lo;
@@ -1094,9 +1125,9 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
             for (uint32_t k = 0; k + 1 < mine; k++) work(k, std::true_type());
             work(mine - 1, std::false_type());
         }
-        if constexpr (TYPE == FHIP_F16 || TYPE == FHIP_Q8_0) {
+        if constexpr (P::UP != 1.f) {
 #pragma unroll
-            for (int j = 0; j < NJ; j++) acc[j] *= TYPE == FHIP_F16 ? 1.f / 32768.f : 1.f / 128.f;
+            for (int j = 0; j < NJ; j++) acc[j] *= 1.f / P::UP;
         }
 
         // the waves' shares joined; element r of acc[j] is dim dim_of(j, 4 kg + r) of head n

@@ -541,8 +541,9 @@ __global__ __launch_bounds__(T) void select_kernel(PagedView kv, const uint32_t*
 //   Q8_0   keys as f16 holds their codes, q as for f16, a block of 32 dims an instruction, whose sum is multiplied by the block's scale; values c * d, 8 by 11 bits, as the two f16 values
 //          whose sum they are, p times 2^15 as two (three products: the two small parts' is 2^-22 of the result). On the f32 instruction, which takes four keys where
 //          these take 32, a capped window of 33 sequences, 16 heads of 64, took 69 us.
-// A step that f16 cannot hold, which a scale of 512 and more makes of Q8_0 values, takes values and weights as three bf16 values each. us, such a scale in every step | in none: Q8_0, 64 sequences
-// of 2000 keys, 8 KV heads of 128 with 5 queries 91 | 62, one of 65536 with 8 queries 57 | 39.
+// What two f16 values do not hold -- weights below 2^-18 of the largest so far, and Q8_0 values whose scale is 512 or more -- takes a step of
+// these types to three bf16 values each, which have f32's range. us, every step so | none: 64 sequences of 2000 keys, 8 KV heads of 128 with 5 queries, Q8_0 75 | 62, f16 101 | 99; heads of 64, Q8_0
+// 44 | 32, f16 46 | 44; one sequence of 65536 with 8 queries of 128, Q8_0 48 | 39, f16 50 | 49.
 // Bound by the rows' bytes. The next step's keys are requested once the current ones are multiplied, its values once the current ones are: eight waves a CU keep 64 KB and more
 // on the way without a second set of registers.
 //
@@ -675,7 +676,7 @@ __device__ __forceinline__ uint32_t xcd_neighbours(uint32_t b, uint32_t n) {
 }
 
 template <int TYPE, int HD, bool SEL, int WV>
-__global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
+__global__ __launch_bounds__(64 * WV, HD == 64 ? 3 : 2) void attention_kernel(Attend a) {
     typedef Path<TYPE> P;
     constexpr int TILES = P::TILES, PARTS = P::PARTS, NB = HD / 32, NJ = HD / 16;
     constexpr int IDS = 64 / TILES;                   // steps whose pages a wave looks up at once
@@ -985,6 +986,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
 #pragma unroll
                     for (int r = 0; r < 4; r++) s[i][r] *= c2;
             }
+            float least = INFINITY;                   // of the keys that count
 #pragma unroll
             for (int i = 0; i < TILES; i++)
                 if (cur[i].pos == NO_PAGE || cur[i].pos + 16 > sp.len || cur[i].pos < sp.lo) {
@@ -997,8 +999,13 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                             else
 #pragma unroll
                                 for (int e = 0; e < VW; e++) vr[i][r][e] = 0;
+                        } else {
+                            least = fminf(least, s[i][r]);
                         }
                     }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) least = fminf(least, s[i][r]);
                 }
             float top = s[0][0];
 #pragma unroll
@@ -1024,7 +1031,7 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                 }
             // weighted rows
             if constexpr (P::HALF) {
-                // p as PARTS 16-bit values each
+                // weights as so many 16-bit values each
                 auto cut_weights = [&](auto bf, auto& pp) {
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
@@ -1034,16 +1041,23 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                         for (int e = 0; e < (int)(sizeof(pp) / sizeof(Frag)); e++) pp[e].w[x] = w[e];
                     }
                 };
+                uint64_t beyond = 0;                         // lanes with something that two f16 values do not hold:
                 uint32_t d2[TYPE == FHIP_Q8_0 ? 4 : 1];      // Q8_0: the scales of keys 2 x and 2 x + 1 in the lane's order
-                if constexpr (TYPE == FHIP_Q8_0) {
-                    u16x2 most = {0, 0};
+                if constexpr (TYPE != FHIP_BF16) {
+                    bool here = least - base < -18.f;        // a weight below 2^-18, whose second part would be smaller than f16's 2^-14, or
+                    if constexpr (TYPE == FHIP_Q8_0) {
+                        u16x2 most = {0, 0};
 #pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        d2[x] = (uint32_t)vd[x / 2][2 * (x & 1)] | (uint32_t)vd[x / 2][2 * (x & 1) + 1] << 16;
-                        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, d2[x]));
+                        for (int x = 0; x < 4; x++) {
+                            d2[x] = (uint32_t)vd[x / 2][2 * (x & 1)] | (uint32_t)vd[x / 2][2 * (x & 1) + 1] << 16;
+                            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, d2[x]));
+                        }
+                        here |= most.x > 0x5FFFu || most.y > 0x5FFFu;      // the values of a scale of 512 and more (or no number)
                     }
-                    if (__any(most.x > 0x5FFFu || most.y > 0x5FFFu)) {      // 512 and more (or no number): c * d would leave f16
-                        // Values and weights as three bf16 values each, which have f32's range: all of their products but that of the smallest (2^-30 of the whole).
+                    beyond = __ballot(here);
+                    if (beyond) {
+                        // weights as three bf16 values each, values as two (f16) or three: all of their products but that of the smallest of three (2^-30 of the whole)
+                        constexpr int VALUE_PARTS = TYPE == FHIP_Q8_0 ? 3 : 2;
                         Frag pp[3];
                         cut_weights(std::true_type(), pp);
 #pragma unroll
@@ -1051,11 +1065,16 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                             float v[8];               // of the lane's keys
 #pragma unroll
                             for (int e = 0; e < 8; e++) {
-                                const f16x2 d = __builtin_bit_cast(f16x2, d2[e / 2]);
-                                v[e] = (float)(int8_t)(vr[e / 4][e % 4][j / 4] >> 8 * (j % 4)) * (float)(e & 1 ? d.y : d.x);
+                                if constexpr (TYPE == FHIP_Q8_0) {
+                                    const f16x2 d = __builtin_bit_cast(f16x2, d2[e / 2]);
+                                    v[e] = (float)(int8_t)(vr[e / 4][e % 4][j / 4] >> 8 * (j % 4)) * (float)(e & 1 ? d.y : d.x);
+                                } else {
+                                    // (of a vector's two the compiler would keep both, for every row: 49 registers spilled)
+                                    v[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(vr[e / 4][e % 4][j / 2] >> 16 * (j & 1)));
+                                }
                             }
 #pragma unroll
-                            for (int b = 0; b < 3; b++) {
+                            for (int b = 0; b < VALUE_PARTS; b++) {
                                 Frag f;
 #pragma unroll
                                 for (int x = 0; x < 4; x++) f.w[x] = upper_halves(__float_as_uint(v[2 * x]), __float_as_uint(v[2 * x + 1]));
@@ -1065,40 +1084,38 @@ __global__ __launch_bounds__(64 * WV, 2) void attention_kernel(Attend a) {
                                 for (int e = 0; e < 8; e++) v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xFFFF0000u);
                             }
                         }
-                        // and nothing is left for the other way (as one of two ways it would cost every step a fifth more registers)
+                    }
+                    // (two branches: of one with two ways the compiler keeps a set of accumulators each, which costs heads of 64 the third wave of a SIMD)
+                    asm volatile("" : "+s"(beyond));
+                }
+                if (!beyond) {
+                    Frag pp[PARTS];
+                    cut_weights(std::integral_constant<bool, TYPE == FHIP_BF16>(), pp);
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) {
+                        Frag f, lo;
 #pragma unroll
                         for (int x = 0; x < 4; x++) {
-                            d2[x] = 0;
-                            p[x / 2][2 * (x & 1)] = p[x / 2][2 * (x & 1) + 1] = 0.f;
+                            const int i = x / 2, r = 2 * (x & 1);
+                            if constexpr (TYPE == FHIP_Q8_0) {
+                                // values j of two keys: c * d = f + lo, exactly
+                                const uint32_t both = __builtin_amdgcn_perm(vr[i][r + 1][j / 4] ^ 0x80808080u, vr[i][r][j / 4] ^ 0x80808080u, (uint32_t)(j % 4) | (uint32_t)(4 + j % 4) << 16 | 0x0C000C00u);
+                                const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
+                                const f16x2 c = __builtin_bit_cast(f16x2, both | 0x64006400u) - off, d = __builtin_bit_cast(f16x2, d2[x]);
+                                const f16x2 hi = c * d;
+                                f.w[x] = __builtin_bit_cast(uint32_t, hi);
+                                lo.w[x] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, d, -hi));
+                            } else {
+                                const uint32_t u = vr[i][r][j / 2], w = vr[i][r + 1][j / 2];
+                                f.w[x] = j & 1 ? upper_halves(u, w) : lower_halves(u, w);
+                            }
                         }
-                    }
-                }
-                Frag pp[PARTS];
-                cut_weights(std::integral_constant<bool, TYPE == FHIP_BF16>(), pp);
+                        if constexpr (TYPE == FHIP_Q8_0) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo.h, pp[0].h, acc[j], 0, 0, 0);
 #pragma unroll
-                for (int j = 0; j < NJ; j++) {
-                    Frag f, lo;
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        const int i = x / 2, r = 2 * (x & 1);
-                        if constexpr (TYPE == FHIP_Q8_0) {
-                            // values j of two keys: c * d = f + lo, exactly
-                            const uint32_t both = __builtin_amdgcn_perm(vr[i][r + 1][j / 4] ^ 0x80808080u, vr[i][r][j / 4] ^ 0x80808080u, (uint32_t)(j % 4) | (uint32_t)(4 + j % 4) << 16 | 0x0C000C00u);
-                            const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
-                            const f16x2 c = __builtin_bit_cast(f16x2, both | 0x64006400u) - off, d = __builtin_bit_cast(f16x2, d2[x]);
-                            const f16x2 hi = c * d;
-                            f.w[x] = __builtin_bit_cast(uint32_t, hi);
-                            lo.w[x] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, d, -hi));
-                        } else {
-                            const uint32_t u = vr[i][r][j / 2], w = vr[i][r + 1][j / 2];
-                            f.w[x] = j & 1 ? upper_halves(u, w) : lower_halves(u, w);
+                        for (int e = PARTS - 1; e >= 0; e--) {
+                            if constexpr (TYPE == FHIP_BF16) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.b, pp[e].b, acc[j], 0, 0, 0);
+                            else acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, pp[e].h, acc[j], 0, 0, 0);
                         }
-                    }
-                    if constexpr (TYPE == FHIP_Q8_0) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo.h, pp[0].h, acc[j], 0, 0, 0);
-#pragma unroll
-                    for (int e = PARTS - 1; e >= 0; e--) {
-                        if constexpr (TYPE == FHIP_BF16) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.b, pp[e].b, acc[j], 0, 0, 0);
-                        else acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.h, pp[e].h, acc[j], 0, 0, 0);
                     }
                 }
             } else {

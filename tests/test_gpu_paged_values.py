@@ -49,3 +49,53 @@ def test_large_scales_beside_small_ones(F, paged, hd, n_kv, g):  # noqa: F811
     q = q.reshape(len(lens), -1)
     out = case.cache.attention(tensor(F, q), words(lens), max(lens), n_kv * g).to_vec()
     check_attention(case, out, q, n_kv * g, lambda i: range(lens[i]))
+
+
+# ---- weights far apart --------------------------------------------------------------------------------------------------------------
+
+def with_a_key_ahead(F, paged, ty, lens, n_kv, g, hd, gap, seed):
+    """A cache in which one key of every sequence and KV head is `gap` nats (and a few) ahead of all others and has a value row of zeros, so that a result is what the others leave; and queries."""
+    rng = np.random.default_rng(seed)
+    case = Filled(F, paged, ty, lens, n_kv, hd, 32, seed)
+    ahead = rng.standard_normal((n_kv, hd))
+    ahead /= np.linalg.norm(ahead, axis=-1, keepdims=True)
+    q = (rng.standard_normal((len(lens), n_kv, g, hd)) + 6 * ahead[:, None]).astype(np.float32)
+    for i, n in enumerate(lens):
+        first = int(rng.integers(n))
+        put(case, "k", i, [first], ((gap + 4) * np.sqrt(hd) / 6 * ahead).reshape(1, -1).astype(np.float32))
+        put(case, "v", i, [first], np.zeros((1, n_kv * hd), np.float32))
+    return case, q.reshape(len(lens), -1)
+
+
+@typed
+@pytest.mark.parametrize("hd,n_kv,g", [(64, 2, 3), (128, 2, 5), (128, 1, 16)])
+@pytest.mark.parametrize("gap", [6, 10, 14, 18, 25, 40, 75])
+def test_weights_far_below_the_largest(F, paged, ty, hd, n_kv, g, gap):  # noqa: F811
+    lens = [40, 33, 700, 3001]
+    case, q = with_a_key_ahead(F, paged, ty, lens, n_kv, g, hd, gap, gap + hd)
+    out = case.cache.attention(tensor(F, q), words(lens), max(lens), n_kv * g).to_vec()
+    check_attention(case, out, q, n_kv * g, lambda i: range(lens[i]))
+
+
+@typed
+def test_weights_far_below_the_largest_over_chosen_pages(F, paged, ty):  # noqa: F811
+    lens, n_kv, g, hd = [3001, 90], 2, 4, 128
+    case, q = with_a_key_ahead(F, paged, ty, lens, n_kv, g, hd, 25, 3)
+    pages = max(-(-n // case.R) for n in lens)
+    listed = np.full((2, n_kv, pages), P.NO_PAGE, np.uint32)
+    for i, n in enumerate(lens):
+        listed[i, :, :-(-n // case.R)] = np.random.default_rng(i).permutation(-(-n // case.R))
+    sel = F.Tensor(words(listed.reshape(-1)).buf, listed.shape, np.uint32)
+    out = case.cache.attention_selected(tensor(F, q), words(lens), sel, n_kv * g).to_vec()
+    check_attention(case, out, q, n_kv * g, lambda i: range(lens[i]))
+
+
+@typed
+@pytest.mark.parametrize("std", [3.0, 9.0])
+def test_scores_of_a_wide_spread(F, paged, ty, std):  # noqa: F811
+    """Weights of every size from the largest down to nothing, in every step."""
+    lens = [1, 100, 513, 2000]
+    case = Filled(F, paged, ty, lens, 2, 64, 16, 7)
+    q = (std * np.random.default_rng(8).standard_normal((len(lens), 6 * 64))).astype(np.float32)
+    out = case.cache.attention(tensor(F, q), words(lens), max(lens), 6).to_vec()
+    check_attention(case, out, q, 6, lambda i: range(lens[i]))

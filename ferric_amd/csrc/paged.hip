@@ -1340,23 +1340,29 @@ constexpr int LOG_WGS = 9, MIN_STEPS = 6;
 // 64 of 500 28.6 | 33.2, 64 of 2000 97.9 | 103, but 8 of 2000 24.5 | 20.1.
 static bool own_workgroups(uint32_t type, const PagedView& kv, size_t keys) {
     const size_t steps = (keys + (type == FHIP_F32 ? 15 : 31)) / (type == FHIP_F32 ? 16 : 32);
-    if ((steps + UNIT_COST) * kv.n_seq * kv.n_kv >= (size_t)1 << 31) return true;      // the deal counts in 32 bits
     return steps <= 16 || ((size_t)kv.n_seq * kv.n_kv >= ((size_t)1 << LOG_WGS) && steps <= 64);
 }
+// The deal counts in 32 bits.
+static bool too_many_steps(uint32_t type, const PagedView& kv, size_t keys) {
+    return (keys / (type == FHIP_F32 ? 16 : 32) + 1 + UNIT_COST) * kv.n_seq * kv.n_kv >= (size_t)1 << 31;
+}
+// The bound on a sequence's keys, which may be anything, as far as the table reaches.
+static size_t within_table(const PagedView& kv, size_t keys) { return keys < (size_t)kv.pages_per_seq << kv.shift ? keys : (size_t)kv.pages_per_seq << kv.shift; }
 static size_t plan_floats(const PagedView& kv) { return ((size_t)kv.n_seq * kv.n_kv + 3) / 4 * 4; }
+// (of a bound with too many steps as of any other: what a bound needs is enough for every smaller one)
 size_t paged_attention_ws_bytes(uint32_t type, const PagedView& kv, int hd, int n_head, size_t max_len) {
-    return own_workgroups(type, kv, max_len) ? 0 : (plan_floats(kv) + ((size_t)2 << LOG_WGS) * (n_head / kv.n_kv) * (hd + 4)) * sizeof(float);
+    return own_workgroups(type, kv, within_table(kv, max_len)) ? 0 : (plan_floats(kv) + ((size_t)2 << LOG_WGS) * (n_head / kv.n_kv) * (hd + 4)) * sizeof(float);
 }
 int launch_paged_attention(uint32_t type, int hd, const PagedView& kv, const float* q, const uint32_t* lens, uint32_t max_len, const uint32_t* selected, uint32_t n_select,
                            int n_head, uint32_t window, float softcap, float* ws, float* out, hipStream_t s) {
     const size_t units = (size_t)kv.n_seq * kv.n_kv;
-    const size_t bound = selected ? (size_t)n_select << kv.shift : max_len;
+    const size_t bound = within_table(kv, selected ? (size_t)n_select << kv.shift : max_len);
     size_t keys = bound;
     if (window > 0 && (size_t)window + 31 < keys) keys = (size_t)window + 31;      // a window begins and ends within steps
     Attend a;
     a.kv = kv; a.q = q; a.lens = lens; a.selected = selected; a.out = out; a.plan = (uint32_t*)ws; a.part = ws + plan_floats(kv);
     a.max_len = max_len; a.n_select = n_select; a.window = window; a.n_head = n_head; a.softcap = softcap; a.scale = 1.0f / sqrtf((float)hd);
-    a.log_wgs = own_workgroups(type, kv, keys) || own_workgroups(type, kv, bound) ? -1 : LOG_WGS;      // (the latter: the caller may have no workspace)
+    a.log_wgs = own_workgroups(type, kv, keys) || own_workgroups(type, kv, bound) || too_many_steps(type, kv, keys) ? -1 : LOG_WGS;      // (the second: the caller may have no workspace)
     a.min_steps = MIN_STEPS;
     const bool alone = a.log_wgs < 0 && units > 4 * (size_t)device_cus();      // more units than the chip has waves for by fours: a wave each
     const dim3 grid(a.log_wgs < 0 ? (unsigned)units : 1u << LOG_WGS);

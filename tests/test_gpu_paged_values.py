@@ -99,3 +99,27 @@ def test_scores_of_a_wide_spread(F, paged, ty, std):  # noqa: F811
     q = (std * np.random.default_rng(8).standard_normal((len(lens), 6 * 64))).astype(np.float32)
     out = case.cache.attention(tensor(F, q), words(lens), max(lens), 6).to_vec()
     check_attention(case, out, q, 6, lambda i: range(lens[i]))
+
+
+# ---- a bound that says nothing ------------------------------------------------------------------------------------------------------
+
+@typed
+def test_no_bound_is_the_table_s_reach(F, paged, ty):  # noqa: F811
+    """The same way of working, so the same bits: two sequences of eight KV heads, long enough that their steps are dealt out; over all rows and over chosen pages."""
+    lens, n_kv, hd = [9000, 8000], 8, 64
+    case = Filled(F, paged, ty, lens, n_kv, hd, 16, 1)
+    reach = case.entries * 16
+    q = np.random.default_rng(0).standard_normal((2, 2 * n_kv * hd)).astype(np.float32)
+    qt, lt = tensor(F, q), words(lens)
+    want = case.cache.attention(qt, lt, reach, 2 * n_kv).to_vec()
+    check_attention(case, want, q, 2 * n_kv, lambda i: range(lens[i]))
+    for bound in (2 ** 32 - 1, 2 ** 40):
+        assert np.array_equal(case.cache.attention(qt, lt, bound, 2 * n_kv).to_vec().view(np.uint32), want.view(np.uint32))
+    got = []
+    for n in (case.entries, 300000):                           # (the list's rows are as many words apart)
+        listed = np.full((2, n_kv, n), P.NO_PAGE, np.uint32)
+        listed[:, :, :case.entries] = np.arange(case.entries)
+        sel = F.Tensor(words(listed.reshape(-1)).buf, listed.shape, np.uint32)
+        got.append(case.cache.attention_selected(qt, lt, sel, 2 * n_kv).to_vec())
+    assert np.array_equal(got[0].view(np.uint32), got[1].view(np.uint32))
+    check_attention(case, got[0], q, 2 * n_kv, lambda i: range(lens[i]))

@@ -470,8 +470,10 @@ int fhip_paged_append(const fhip_paged* kv, const float* d_qkv, const float* d_b
 /* One new token of every sequence: q [n_seq, n_head * head_dim] against the first d_lens[i] rows of sequence i (the token's own among them), or the newest `window` of these when
  * window > 0; softcap as fhip_decode_attention_ex. out[i, h] = softmax_j(q . K_j / sqrt(head_dim)) @ V, query head h with KV head h / (n_head / n_kv), n_head a multiple of n_kv up to
  * 16 times it. d_lens is read on the device, so one captured launch serves growing sequences; max_len is the host's bound that sizes the work: a longer length is cut
- * to it and to what the table reaches. A length of 0, or no row left, gives zeros. f32 arithmetic, the rows enter as the values they stand for; the same inputs give the same bits. What lies
- * behind a sequence's last row is never part of a result, whatever it holds; an infinite or NaN value among its rows makes what it enters non-finite (infinite values of 16-bit and Q8_0 rows make NaN). n_seq * n_head
+ * to it and to what the table reaches. A length of 0, or no row left, gives zeros. f32 arithmetic, the rows enter as the values they stand for (queries and weights with 22 bits or more; over
+ * f16 and Q8_0 rows a query's values no finer than 2^-39 of its head's largest); the same inputs give the same bits. What lies behind a sequence's last row is never part of a result, whatever
+ * it holds; among its rows a key that is NaN makes all of its KV head's results NaN, an infinite or NaN value its dim's (Q8_0: that of a scale its block's) infinite or NaN. An infinite key
+ * counts by its score: over f32 rows one of -inf has no weight (under a softcap the cap's), any other infinity, and over the other rows either, may make the KV head's results NaN. n_seq * n_head
  * below 2^23 (FHIP_ERR_SHAPE). d_ws: fhip_paged_attention_ws_bytes(kv, n_head, max_len) bytes of scratch, 16-byte aligned (NULL when
  * that is 0), the call's own until the stream has passed it. */
 size_t fhip_paged_attention_ws_bytes(const fhip_paged* kv, size_t n_head, size_t max_len);

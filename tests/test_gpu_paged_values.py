@@ -123,3 +123,55 @@ def test_no_bound_is_the_table_s_reach(F, paged, ty):  # noqa: F811
         got.append(case.cache.attention_selected(qt, lt, sel, 2 * n_kv).to_vec())
     assert np.array_equal(got[0].view(np.uint32), got[1].view(np.uint32))
     check_attention(case, got[0], q, 2 * n_kv, lambda i: range(lens[i]))
+
+
+# ---- capped, extreme and infinite values --------------------------------------------------------------------------------------------
+
+@typed
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+@pytest.mark.parametrize("far", [False, True])
+def test_infinite_values_stay_in_their_dims(F, paged, ty, value, far):  # noqa: F811
+    """An infinite value (Q8_0: a block's scale) makes its dim (block) of its KV head non-finite and nothing else, also where weights are far apart."""
+    lens, n_kv, g, hd = [200, 33], 2, 3, 64
+    case, q = with_a_key_ahead(F, paged, ty, lens, n_kv, g, hd, 25 if far else 1, 5)
+    want = case.cache.attention(tensor(F, q), words(lens), max(lens), n_kv * g).to_vec().reshape(2, n_kv, g, hd)
+    pool, scales = case.raw["v"]
+    row = P.place(case.table[0], [77], case.R, case.n_pages)[0]
+    if ty == P.Q8_0:
+        scales[row, 1] = value                                 # KV head 0, dims 32 .. 63
+        upload(case.cache.v_scales, scales)
+    else:
+        pool[row, 40] = P.bf16_bits(np.float32(value))[0] if ty == P.BF16 else value
+        upload(case.cache.v, pool)
+    out = case.cache.attention(tensor(F, q), words(lens), max(lens), n_kv * g).to_vec().reshape(2, n_kv, g, hd)
+    hit = np.zeros(out.shape, bool)
+    hit[0, 0, :, 32 if ty == P.Q8_0 else 40:64 if ty == P.Q8_0 else 41] = True
+    assert not np.isfinite(out[hit]).any()
+    # the same step may go another way (a scale that is no number): to f32 arithmetic's allowance, not to the bit
+    q = q.reshape(2, n_kv * g, hd)
+    for i, n in enumerate(lens):
+        k, v = case.values("k", i, range(n)), case.values("v", i, range(n))
+        v[~np.isfinite(v)] = 0
+        _, tol = P.attend(q[i].astype(np.float64), k, v)
+        keep = ~hit[i].reshape(n_kv * g, hd)
+        assert (np.abs(out[i].reshape(n_kv * g, hd) - want[i].reshape(n_kv * g, hd))[keep] <= 2 * tol[keep]).all()
+
+
+@typed
+def test_a_key_that_is_no_number_makes_its_kv_head_s_results_none(F, paged, ty):  # noqa: F811
+    lens, n_kv, g, hd = [200, 33], 2, 3, 128
+    case = Filled(F, paged, ty, lens, n_kv, hd, 32, 6)
+    q = np.random.default_rng(7).standard_normal((2, n_kv * g * hd)).astype(np.float32)
+    want = case.cache.attention(tensor(F, q), words(lens), max(lens), n_kv * g).to_vec().reshape(2, n_kv, g, hd)
+    pool, scales = case.raw["k"]
+    row = P.place(case.table[0], [100], case.R, case.n_pages)[0]
+    if ty == P.Q8_0:
+        scales[row, hd // 32] = np.nan
+        upload(case.cache.k_scales, scales)
+    else:
+        pool[row, hd + 5] = 0x7FC0 if ty == P.BF16 else np.nan
+        upload(case.cache.k, pool)
+    out = case.cache.attention(tensor(F, q), words(lens), max(lens), n_kv * g).to_vec().reshape(2, n_kv, g, hd)
+    assert np.isnan(out[0, 1]).all()
+    out[0, 1] = want[0, 1] = 0
+    assert np.array_equal(out, want)

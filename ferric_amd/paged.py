@@ -116,7 +116,7 @@ class PagedKvCache:
 
     def attention(self, q, lens, max_len, n_heads, window=0, softcap=0.0, out=None, ws=None, stream=None):
         """One new token of every sequence, q [n_seq, n_heads * head_dim], over the first lens[i] rows (device u32 Tensor, the new token's own among them; at most
-        max_len) or the newest `window` of them."""
+        max_len) or the newest `window` of them. ws: scratch of the caller's in place of the cache's own for the stream; memory that does not say its nbytes is taken at the caller's word."""
         out = self._query(q, lens, n_heads, out)
         _lib.paged_attention(self._addr, q.buf, lens.buf, max_len, n_heads, window, softcap, self._workspace(n_heads, max_len, ws, stream), out.buf, _at(stream))
         return out
@@ -153,7 +153,8 @@ class PagedKvCache:
         return out
 
     def rows(self, seq, row0, rows, out=None, stream=None):
-        """Rows row0 .. row0 + rows of sequence seq as f32: (k, v), [rows, n_kv * head_dim] each."""
+        """Rows row0 .. row0 + rows of sequence seq as f32: (k, v), [rows, n_kv * head_dim] each. Rows of a table entry that names no page are not written: they stay as `out` has
+        them, and without `out` hold anything."""
         shape = (rows, self._rows)
         k, v = (Tensor.empty(shape), Tensor.empty(shape)) if out is None else out
         assert k.shape == v.shape == shape, "rows: out has another shape"

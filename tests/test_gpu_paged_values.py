@@ -128,6 +128,38 @@ def test_no_bound_is_the_table_s_reach(F, paged, ty):  # noqa: F811
 # ---- capped, extreme and infinite values --------------------------------------------------------------------------------------------
 
 @typed
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("cap", [0.5, 5.0, 30.0])
+def test_scores_far_past_the_cap(F, paged, ty, hd, cap):  # noqa: F811
+    """Where tanh has nearly reached one, and everything in front of that."""
+    lens = [1, 33, 700]
+    case = Filled(F, paged, ty, lens, 2, hd, 32, 9)
+    q = (10 * np.random.default_rng(4).standard_normal((len(lens), 6 * hd))).astype(np.float32)
+    out = case.cache.attention(tensor(F, q), words(lens), max(lens), 6, softcap=cap).to_vec()
+    check_attention(case, out, q, 6, lambda i: range(lens[i]), cap)
+
+
+@typed
+def test_queries_of_every_size(F, paged, ty):  # noqa: F811
+    """A query head is worked with at a power of two of its own on f16 and Q8_0 rows: heads from nothing to the largest, with keys of ordinary size and of such as bring the scores back."""
+    lens, hd, sizes = [200, 1, 65], 128, [0.0, 1e-44, 1e-38, 1e-20, 1e-3, 1.0, 1e3, 3e38]
+    for std in (1.0, 1e-3, 50.0):
+        case = Filled(F, paged, ty, lens, 1, hd, 16, 11, std=std)
+        q = np.random.default_rng(2).uniform(-1, 1, (len(lens), len(sizes), hd))
+        q = (q * np.array(sizes)[:, None]).astype(np.float32)
+        # scores past f32's largest are infinite in f32 arithmetic: the largest queries have one dim, against keys that are tiny there
+        q[:, -1, 1:] = 0
+        for i, n in enumerate(lens):
+            k = case.values("k", i, range(n)).reshape(n, hd).astype(np.float32)
+            k[:, 0] = 1e-6 * np.sign(k[:, 0])
+            put(case, "k", i, range(n), k)
+        q[:, -1, 0] *= 1e-31
+        q = q.reshape(len(lens), -1)
+        out = case.cache.attention(tensor(F, q), words(lens), max(lens), len(sizes)).to_vec()
+        check_attention(case, out, q, len(sizes), lambda i: range(lens[i]), label=std)
+
+
+@typed
 @pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
 @pytest.mark.parametrize("far", [False, True])
 def test_infinite_values_stay_in_their_dims(F, paged, ty, value, far):  # noqa: F811
@@ -175,3 +207,25 @@ def test_a_key_that_is_no_number_makes_its_kv_head_s_results_none(F, paged, ty):
     assert np.isnan(out[0, 1]).all()
     out[0, 1] = want[0, 1] = 0
     assert np.array_equal(out, want)
+
+
+# ---- one cache on two streams -------------------------------------------------------------------------------------------------------
+
+def test_one_cache_on_two_streams(F, paged):  # noqa: F811
+    """A workspace for each: calls of one cache, dealt out and joined, with other queries and lengths on either stream."""
+    lens = [[30000, 9000], [12000, 25000]]
+    case = Filled(F, paged, P.BF16, [30000, 25000], 2, 128, 64, 1)
+    streams, nh = [F.Stream(), F.Stream()], 8
+    qs = [np.random.default_rng(i).standard_normal((2, nh * 128)).astype(np.float32) for i in range(2)]
+    qt, lt = [tensor(F, q) for q in qs], [words(n) for n in lens]
+    alone = [case.cache.attention(qt[i], lt[i], 30000, nh).to_vec() for i in range(2)]
+    for i in range(2):
+        case.lens = lens[i]
+        check_attention(case, alone[i], qs[i], nh, lambda s, i=i: range(lens[i][s]))
+        case.cache.reserve(nh, 30000, stream=streams[i])
+    kept = [case.cache._workspace(nh, 30000, None, s) for s in streams]
+    assert kept[0].ptr.value != kept[1].ptr.value and case.cache._workspace(nh, 30000, None, None).ptr.value not in (kept[0].ptr.value, kept[1].ptr.value)
+    F._lib.check(F._lib.load().fhip_stream_sync(None))
+    outs = [(i, case.cache.attention(qt[i], lt[i], 30000, nh, stream=streams[i])) for _ in range(20) for i in range(2)]
+    for i, o in outs:
+        assert np.array_equal(o.to_vec(streams[i]).view(np.uint32), alone[i].view(np.uint32))

@@ -542,8 +542,8 @@ __global__ __launch_bounds__(T) void select_kernel(PagedView kv, const uint32_t*
 //          whose sum they are, p times 2^15 as two (three products: the two small parts' is 2^-22 of the result). On the f32 instruction, which takes four keys where
 //          these take 32, a capped window of 33 sequences, 16 heads of 64, took 69 us.
 // What two f16 values do not hold -- weights below 2^-18 of the largest so far, and Q8_0 values whose scale is 512 or more -- takes a step of
-// these types to three bf16 values each, which have f32's range. us, every step so | none: 64 sequences of 2000 keys, 8 KV heads of 128 with 5 queries, Q8_0 75 | 62, f16 101 | 99; heads of 64, Q8_0
-// 44 | 32, f16 46 | 44; one sequence of 65536 with 8 queries of 128, Q8_0 48 | 39, f16 50 | 49.
+// these types to three bf16 values each, which have f32's range. us, every step so | none: 64 sequences of 2000 keys, 8 KV heads of 128 with 5 queries, Q8_0 75 | 62, f16 100 | 99; heads of 64, Q8_0
+// 44 | 33, f16 44 | 44; one sequence of 65536 with 8 queries of 128, Q8_0 48 | 39, f16 50 | 49.
 // Bound by the rows' bytes. The next step's keys are requested once the current ones are multiplied, its values once the current ones are: eight waves a CU keep 64 KB and more
 // on the way without a second set of registers.
 //
